@@ -24,6 +24,7 @@
 #include "fp32_kernels.h"
 #include "internal.h"
 #include "paged_decode.h"
+#include "paged_step.h"
 #include "prefill.h"
 #include "ptx.cuh"
 #include "rope.h"
@@ -491,6 +492,138 @@ int fe_paged_kv_append(const void* k_new, const void* v_new, void* k_cache, void
   if (dtype == 1) return static_cast<int>(fe::paged::launch_kv_append<half>(ap, st));
   if (dtype == 2) return static_cast<int>(fe::paged::launch_kv_append<float>(ap, st));
   return kErr;
+}
+
+// ---- serving step ------------------------------------------------------------------
+int fe_plan_paged_step(const int* context_lens, const int* new_lens,
+                       const unsigned char* finished, int* block_tables, int* free_blocks,
+                       const int* free_state, int* context_lens_out, int* cu_seqlens,
+                       int* positions, long long* slots, int* free_state_out, int S, int maxb,
+                       int num_blocks, int bs, int max_tokens, void* stream) {
+  if (S < 0 || S > fe::step::kMaxPlanSeqs || maxb < 0 || num_blocks < 1 ||
+      num_blocks >= fe::step::kMaxPlanCount || bs < 1 || max_tokens < 0 ||
+      max_tokens >= fe::step::kMaxPlanCount)
+    return kErr;
+  unsigned* err = fe::device_error_word();
+  if (!err) return static_cast<int>(cudaErrorInitializationError);
+  const fe::step::PlanParams p{context_lens, new_lens, finished, block_tables, free_blocks,
+                               free_state, context_lens_out, cu_seqlens, positions, slots,
+                               free_state_out, S, maxb, num_blocks, bs, max_tokens, err};
+  return static_cast<int>(fe::step::launch_plan(p, as_stream(stream)));
+}
+
+int fe_paged_qkv_append(const void* qkv, long long row_stride, void* q_out, void* k_cache,
+                        void* v_cache, const int* positions, const long long* slots,
+                        const void* q_weight, const void* k_weight, int weight_fp32, float eps,
+                        const float* rope_cos, const float* rope_sin, int rotary_dim,
+                        int rope_max_pos, int interleaved, int T, int H, int Hkv, int d, int bs,
+                        int num_blocks, int dtype, int kv_layout, void* stream) {
+  if (T < 0 || H < 1 || Hkv < 1 || d < 1 || bs < 1 || num_blocks < 1 || dtype < 0 || dtype > 2)
+    return kErr;
+  if (row_stride < (static_cast<long long>(H) + 2LL * Hkv) * d || !(eps >= 0.f)) return kErr;
+  if (kv_layout != fe::paged::kKvFlat && kv_layout != fe::paged::kKvVllm) return kErr;
+  if (kv_layout == fe::paged::kKvVllm && (dtype == 2 || d % 8 != 0)) return kErr;
+  if ((rope_cos == nullptr) != (rope_sin == nullptr)) return kErr;
+  if (rope_cos && (rotary_dim < 2 || rotary_dim % 2 != 0 || rotary_dim > d || rope_max_pos < 1))
+    return kErr;
+  if (T == 0) return 0;
+  unsigned* err = fe::device_error_word();
+  if (!err) return static_cast<int>(cudaErrorInitializationError);
+  fe::step::QkvParams p{};
+  p.qkv = qkv;
+  p.q_out = q_out;
+  p.k_cache = k_cache;
+  p.v_cache = v_cache;
+  p.positions = positions;
+  p.slots = slots;
+  p.q_weight = q_weight;
+  p.k_weight = k_weight;
+  p.rope_cos = rope_cos;
+  p.rope_sin = rope_sin;
+  p.row_stride = row_stride;
+  p.eps = eps;
+  p.tokens = T;
+  p.heads = H;
+  p.kv_heads = Hkv;
+  p.head_dim = d;
+  p.block_size = bs;
+  p.num_blocks = num_blocks;
+  p.rotary_dim = rotary_dim;
+  p.rope_max_pos = rope_max_pos;
+  p.interleaved = interleaved;
+  p.weight_f32 = weight_fp32;
+  p.kv_layout = kv_layout;
+  p.err = err;
+  return static_cast<int>(fe::step::launch_qkv_append(p, dtype, as_stream(stream)));
+}
+
+int fe_update_page_bounds(const void* k_cache, signed char* values, float* scales,
+                          const long long* slots, int T, int Hkv, int d, int bs, int num_blocks,
+                          int dtype, int kv_layout, void* stream) {
+  if (T < 0 || Hkv < 1 || num_blocks < 1 || dtype < 0 || dtype > 2) return kErr;
+  if (!(d == 64 || d == 128) || !(bs == 16 || bs == 32)) return kErr;
+  if (kv_layout != fe::paged::kKvFlat && kv_layout != fe::paged::kKvVllm) return kErr;
+  if (kv_layout == fe::paged::kKvVllm && (bs != 16 || dtype == 2)) return kErr;
+  if (!aligned(k_cache, 16) || !aligned(values, 16) || !aligned(scales, 4)) return kErr;
+  if (T == 0) return 0;
+  unsigned* err = fe::device_error_word();
+  if (!err) return static_cast<int>(cudaErrorInitializationError);
+  const fe::step::BoundsParams p{k_cache, values, scales, slots, T, Hkv, num_blocks, kv_layout,
+                                 err};
+  return static_cast<int>(fe::step::launch_page_bounds(p, d, bs, dtype, as_stream(stream)));
+}
+
+int fe_sparse_paged_attention(const void* q, const void* kc, const void* vc, void* out,
+                              const signed char* values, const float* scales, const int* bt,
+                              const int* lens, int* selected, int* scratch, int S, int H, int Hkv,
+                              int d, int bs, int maxb, int num_blocks, int num_pages,
+                              int keep_first, int keep_last, float scale, int dtype,
+                              int kv_layout, float* workspace, size_t workspace_floats,
+                              void* stream) {
+  if (S < 0 || H < 1 || Hkv < 1 || H % Hkv != 0 || num_blocks < 1 || maxb < 1) return kErr;
+  if (keep_first < 0 || keep_last < 1 ||
+      static_cast<long long>(keep_first) + keep_last > num_pages)
+    return kErr;
+  if (!aligned(values, 16) || !aligned(scales, 4)) return kErr;
+  const long long rows = static_cast<long long>(S) * Hkv;
+  if (rows * fe::step::kMaxSelectCtas > INT_MAX || rows * num_pages > INT_MAX ||
+      !fe::step::select_width_ok(maxb, H / Hkv, d))
+    return kErr;
+  // The decode sees every (sequence, KV head) as a sequence of its own with one KV head,
+  // and the cache as num_blocks * Hkv blocks of it: a page of one head is contiguous.
+  const int G = H / Hkv;
+  PagedArgs a{q,  kc, vc, out,       scratch + rows, scratch, static_cast<int>(rows), G, 1, d, bs,
+              0,  num_pages, 0, scale};
+  if (static_cast<long long>(num_blocks) * Hkv * bs > INT_MAX) return kErr;
+  a.num_blocks = num_blocks * Hkv;
+  a.kv_layout = kv_layout;
+  const int rc = dtype == 0 ? paged_check<__nv_bfloat16>(a)
+                 : dtype == 1 ? paged_check<half>(a)
+                 : dtype == 2 ? paged_check<float>(a)
+                              : kErr;
+  if (rc) return rc;
+  const bool lib = !workspace && workspace_floats == FE_WORKSPACE_LIBRARY;
+  if (!lib) {
+    const long long need = workspace_floats_dtype(dtype, G, 1, d, bs);
+    if (need <= 0 || !workspace || static_cast<long long>(workspace_floats) < need) return kErr;
+  }
+  if (S == 0) return 0;
+  unsigned* err = fe::device_error_word();
+  if (!err) return static_cast<int>(cudaErrorInitializationError);
+  cudaStream_t st = as_stream(stream);
+  const fe::step::SelectParams sp{q, values, scales, bt, lens, selected, scratch + rows, scratch,
+                                  S, H, Hkv, maxb, num_blocks, bs, num_pages, keep_first,
+                                  keep_last, err};
+  const cudaError_t e = fe::step::launch_page_select(sp, d, dtype, st);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (dtype == 0)
+    return lib ? paged_v1_entry<__nv_bfloat16>(a, st)
+               : paged_v2_tc<__nv_bfloat16>(a, workspace, workspace_floats, st);
+  if (dtype == 1)
+    return lib ? paged_v1_entry<half>(a, st)
+               : paged_v2_tc<half>(a, workspace, workspace_floats, st);
+  return lib ? paged_v1_entry<float>(a, st)
+             : paged_v2_tc<float>(a, workspace, workspace_floats, st);
 }
 
 size_t fe_paged_attention_v2_workspace_floats(int H, int Hkv, int d, int bs) {

@@ -19,6 +19,15 @@ from .ops import (  # noqa: F401
     paged_kv_append,
     rope,
 )
+from .step import (  # noqa: F401
+    PageBounds,
+    PagedStep,
+    new_page_bounds,
+    paged_qkv_append,
+    plan_paged_step,
+    sparse_paged_attention,
+    update_page_bounds,
+)
 
 __version__ = "1.2.0"
 
@@ -31,6 +40,13 @@ __all__ = [
     "paged_kv_append",
     "rope",
     "merge_partials",
+    "plan_paged_step",
+    "PagedStep",
+    "paged_qkv_append",
+    "PageBounds",
+    "new_page_bounds",
+    "update_page_bounds",
+    "sparse_paged_attention",
     "paged_attention_workspace_floats",
     "device_errors",
     "get_version",

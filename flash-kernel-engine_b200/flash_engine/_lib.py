@@ -68,6 +68,11 @@ _SIGS = {
     "fe_paged_decode_kv_range_nccl_bf16": ([_P] * 5 + [_I] * 7 + [_F, _I, _P, ctypes.c_size_t,
                                                                    _P, _I, _I, _P, ctypes.c_size_t,
                                                                    _P, _P], _I),
+    "fe_plan_paged_step": ([_P] * 11 + [_I] * 5 + [_P], _I),
+    "fe_paged_qkv_append": ([_P, _LL] + [_P] * 7 + [_I, _F, _P, _P] + [_I] * 11 + [_P], _I),
+    "fe_update_page_bounds": ([_P] * 4 + [_I] * 7 + [_P], _I),
+    "fe_sparse_paged_attention": ([_P] * 10 + [_I] * 10 + [_F, _I, _I, _P, ctypes.c_size_t, _P],
+                                  _I),
     "fe_graph_capture": ([None, _P, _P, ctypes.POINTER(ctypes.c_void_p)], _I),
     "fe_graph_launch": ([_P, _P], _I),
     "fe_graph_destroy": ([_P], None),

@@ -384,6 +384,91 @@ int fe_paged_decode_kv_range_nccl_bf16(const void* q, const void* k_cache, const
                                        int rank, int world, float* scratch,
                                        size_t scratch_floats, void* out, void* stream);
 
+/* ---------------------------------------------------------------- serving step
+ * What a serving step does around the paged decode: the plan (blocks, slots), the QKV
+ * append (QK norm, rotary embedding, cache write), the page boxes, and decode attention
+ * over the pages the boxes select. New: the reference has none of these. */
+
+/* Block tables, positions and cache slots of one step from request lengths that live on
+ * the GPU. Request s holds context_lens[s] tokens and adds new_lens[s] (negative = 0);
+ * finished (may be NULL): one byte a request, non-zero = its blocks go back to the ring
+ * and its row starts again at length 0 (with new_lens[s] > 0 the row is reused at once;
+ * blocks given back serve from the next step on). The free blocks are a ring:
+ * free_blocks[(head + i) % num_blocks], i < count, free_state = (head, count).
+ * Requests are served in order until one does not fit: its tokens in max_tokens, its
+ * blocks in count, its length in max_blocks_per_seq * block_size. That one and every
+ * later one get no tokens. Outputs:
+ *   context_lens_out [S]    tokens held after the step
+ *   cu_seqlens [S + 1]      first token of each request; cu_seqlens[S] = tokens
+ *   positions [max_tokens]  position of each token in its request, -1 past the tokens
+ *   slots [max_tokens]      block * block_size + offset, -1 past the tokens
+ *   free_state_out [4]      (head, count, requests served, tokens)
+ * block_tables and free_blocks are updated in place; context_lens_out may not be
+ * context_lens, free_state_out may be neither free_state nor any other input. At most
+ * 16384 requests; max_tokens and num_blocks below 2^30. A ring that would hold more than
+ * num_blocks sets bit 1 of the device error word. */
+int fe_plan_paged_step(const int* context_lens, const int* new_lens,
+                       const unsigned char* finished, int* block_tables, int* free_blocks,
+                       const int* free_state, int* context_lens_out, int* cu_seqlens,
+                       int* positions, long long* slots, int* free_state_out, int num_seqs,
+                       int max_blocks_per_seq, int num_blocks, int block_size, int max_tokens,
+                       void* stream);
+
+/* One pass over a step's QKV projection: qkv [tokens, (heads + 2 kv_heads) head_dim], rows
+ * row_stride elements apart, query heads first, then key and value heads.
+ *   - per-head RMS norm of queries (q_weight) and keys (k_weight), weights [head_dim] of
+ *     the data's type or fp32 (weight_fp32), NULL = no norm of that part;
+ *   - rotary embedding of both at positions[t] (rope_cos / rope_sin NULL = off): fp32
+ *     tables [rope_max_pos, rotary_dim / 2], pairs (2i, 2i+1) with interleaved, else
+ *     (i, i + rotary_dim / 2), over the first rotary_dim elements;
+ *   - queries to q_out [tokens, heads, head_dim], keys and values to cache slots
+ *     slots[t] = block * block_size + offset.
+ * A token with position < 0 is padding: zero query row, nothing cached. slots[t] < 0: not
+ * cached. A position past the tables (its token is then padding) or a slot past num_blocks
+ * sets bit 1 of the device error word. dtype 0 bf16, 1 fp16, 2 fp32; kv_layout 0 flat,
+ * 1 vLLM (16-bit types, head_dim % 8 == 0). Any head_dim; 64, 128 and 256 with 16-byte
+ * aligned rows and full rotation take the vector path. q_out may not overlap qkv. */
+int fe_paged_qkv_append(const void* qkv, long long row_stride, void* q_out, void* k_cache,
+                        void* v_cache, const int* positions, const long long* slots,
+                        const void* q_weight, const void* k_weight, int weight_fp32, float eps,
+                        const float* rope_cos, const float* rope_sin, int rotary_dim,
+                        int rope_max_pos, int interleaved, int tokens, int heads, int kv_heads,
+                        int head_dim, int block_size, int num_blocks, int dtype, int kv_layout,
+                        void* stream);
+
+/* int8 boxes of the keys of the pages that the tokens with these slots filled (the slot at
+ * a page's last place closes it; other slots are skipped). For page b and KV head h:
+ * scales[b, h] = 2^e with the smallest e >= -120 for which every |key| <= 127 * 2^e, and
+ * values[b, h] = int8 [2, head_dim]: ceil(largest / 2^e), then floor(smallest / 2^e), per
+ * channel. A page with a NaN or an infinity gets zeros and the scale +inf. values
+ * [num_blocks, kv_heads, 2, head_dim], 16-byte aligned; scales [num_blocks, kv_heads] fp32.
+ * head_dim 64 or 128, block_size 16 or 32, dtype and kv_layout as for fe_paged_qkv_append
+ * (vLLM: block_size 16). */
+int fe_update_page_bounds(const void* k_cache, signed char* values, float* scales,
+                          const long long* slots, int tokens, int kv_heads, int head_dim,
+                          int block_size, int num_blocks, int dtype, int kv_layout,
+                          void* stream);
+
+/* Paged decode attention over num_pages pages of each (sequence, KV head): the first
+ * keep_first and the last keep_last (>= 1) pages and those whose boxes bound q.k highest
+ * (over the group's query heads; the query rounded to whole numbers like a box; ties to
+ * the lower page). A sequence of at most num_pages pages is attended whole. num_pages >=
+ * keep_first + keep_last. Boxes are read for full pages only that are neither the first
+ * keep_first nor the last keep_last ones. q, caches, tables, lengths, scale, dtype,
+ * kv_layout and the workspace are those of fe_paged_attention_ex; num_blocks must be
+ * given, scale is positive. Outputs: out [S, H, d]; selected [S, Hkv, num_pages], the
+ * chosen page indices in ascending order, -1 past their count. scratch: S * Hkv *
+ * (num_pages + 1) ints. Two launches: the selection, and the decode with a block table for
+ * each (sequence, KV head). */
+int fe_sparse_paged_attention(const void* q, const void* k_cache, const void* v_cache, void* out,
+                              const signed char* values, const float* scales,
+                              const int* block_tables, const int* context_lens, int* selected,
+                              int* scratch, int num_seqs, int num_heads, int num_kv_heads,
+                              int head_dim, int block_size, int max_blocks_per_seq,
+                              int num_blocks, int num_pages, int keep_first, int keep_last,
+                              float scale, int dtype, int kv_layout, float* workspace,
+                              size_t workspace_floats, void* stream);
+
 /* ---------------------------------------------------------------- CUDA graphs
  * Capture-once / replay-per-step of a decode step (kernels, merges and -- when the
  * recorded function issues them -- NCCL collectives). Wraps the CUDAGraphRunner of
