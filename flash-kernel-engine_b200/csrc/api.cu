@@ -504,6 +504,10 @@ int fe_plan_paged_step(const int* context_lens, const int* new_lens,
       num_blocks >= fe::step::kMaxPlanCount || bs < 1 || max_tokens < 0 ||
       max_tokens >= fe::step::kMaxPlanCount)
     return kErr;
+  if (!free_blocks || !free_state || !cu_seqlens || !free_state_out ||
+      (S > 0 && (!context_lens || !new_lens || !context_lens_out || (maxb > 0 && !block_tables))) ||
+      (max_tokens > 0 && (!positions || !slots)))
+    return kErr;
   unsigned* err = fe::device_error_word();
   if (!err) return static_cast<int>(cudaErrorInitializationError);
   const fe::step::PlanParams p{context_lens, new_lens, finished, block_tables, free_blocks,
@@ -527,6 +531,7 @@ int fe_paged_qkv_append(const void* qkv, long long row_stride, void* q_out, void
   if (rope_cos && (rotary_dim < 2 || rotary_dim % 2 != 0 || rotary_dim > d || rope_max_pos < 1))
     return kErr;
   if (T == 0) return 0;
+  if (!qkv || !q_out || !k_cache || !v_cache || !positions || !slots) return kErr;
   unsigned* err = fe::device_error_word();
   if (!err) return static_cast<int>(cudaErrorInitializationError);
   fe::step::QkvParams p{};
@@ -566,6 +571,7 @@ int fe_update_page_bounds(const void* k_cache, signed char* values, float* scale
   if (kv_layout == fe::paged::kKvVllm && (bs != 16 || dtype == 2)) return kErr;
   if (!aligned(k_cache, 16) || !aligned(values, 16) || !aligned(scales, 4)) return kErr;
   if (T == 0) return 0;
+  if (!k_cache || !values || !scales || !slots) return kErr;
   unsigned* err = fe::device_error_word();
   if (!err) return static_cast<int>(cudaErrorInitializationError);
   const fe::step::BoundsParams p{k_cache, values, scales, slots, T, Hkv, num_blocks, kv_layout,
@@ -586,14 +592,15 @@ int fe_sparse_paged_attention(const void* q, const void* kc, const void* vc, voi
     return kErr;
   if (!aligned(values, 16) || !aligned(scales, 4)) return kErr;
   const long long rows = static_cast<long long>(S) * Hkv;
-  if (rows * fe::step::kMaxSelectCtas > INT_MAX || rows * num_pages > INT_MAX ||
-      !fe::step::select_width_ok(maxb, H / Hkv, d))
+  const bool two = fe::step::sparse_two_pass(maxb);
+  if (rows * 8 > INT_MAX || rows * (num_pages + 1LL) > INT_MAX || H / Hkv > 128 ||
+      (two && rows * ((maxb + 255LL) / 256) > INT_MAX))
     return kErr;
   // The decode sees every (sequence, KV head) as a sequence of its own with one KV head,
   // and the cache as num_blocks * Hkv blocks of it: a page of one head is contiguous.
   const int G = H / Hkv;
-  PagedArgs a{q,  kc, vc, out,       scratch + rows, scratch, static_cast<int>(rows), G, 1, d, bs,
-              0,  num_pages, 0, scale};
+  PagedArgs a{q, kc, vc, out, scratch + rows, scratch, static_cast<int>(rows), G, 1, d, bs, 0,
+              num_pages, 0, scale};
   if (static_cast<long long>(num_blocks) * Hkv * bs > INT_MAX) return kErr;
   a.num_blocks = num_blocks * Hkv;
   a.kv_layout = kv_layout;
@@ -608,14 +615,38 @@ int fe_sparse_paged_attention(const void* q, const void* kc, const void* vc, voi
     if (need <= 0 || !workspace || static_cast<long long>(workspace_floats) < need) return kErr;
   }
   if (S == 0) return 0;
+  if (!q || !kc || !vc || !out || !values || !scales || !bt || !lens || !selected || !scratch)
+    return kErr;
   unsigned* err = fe::device_error_word();
   if (!err) return static_cast<int>(cudaErrorInitializationError);
   cudaStream_t st = as_stream(stream);
-  const fe::step::SelectParams sp{q, values, scales, bt, lens, selected, scratch + rows, scratch,
-                                  S, H, Hkv, maxb, num_blocks, bs, num_pages, keep_first,
-                                  keep_last, err};
-  const cudaError_t e = fe::step::launch_page_select(sp, d, dtype, st);
-  if (e != cudaSuccess) return static_cast<int>(e);
+  fe::step::SelectParams sp{};
+  sp.q = q;
+  sp.k_cache = kc;
+  sp.v_cache = vc;
+  sp.out = out;
+  sp.values = values;
+  sp.scales = scales;
+  sp.block_tables = bt;
+  sp.context_lens = lens;
+  sp.selected = selected;
+  sp.sel_lens = scratch;
+  sp.sel_blocks = scratch + rows;
+  sp.keys = two ? reinterpret_cast<unsigned*>(scratch + rows * (num_pages + 1LL)) : nullptr;
+  sp.num_seqs = S;
+  sp.heads = H;
+  sp.kv_heads = Hkv;
+  sp.width = maxb;
+  sp.num_blocks = num_blocks;
+  sp.block_size = bs;
+  sp.num_pages = num_pages;
+  sp.keep_first = keep_first;
+  sp.keep_last = keep_last;
+  sp.scale_log2 = resolve_scale(scale, d) * fe::kLog2e;
+  sp.err = err;
+  const bool fused = fe::step::sparse_fused(sp, dtype, kv_layout);
+  const cudaError_t e = fe::step::launch_sparse(sp, d, dtype, fused, st);
+  if (e != cudaSuccess || fused) return static_cast<int>(e);
   if (dtype == 0)
     return lib ? paged_v1_entry<__nv_bfloat16>(a, st)
                : paged_v2_tc<__nv_bfloat16>(a, workspace, workspace_floats, st);
@@ -624,6 +655,13 @@ int fe_sparse_paged_attention(const void* q, const void* kc, const void* vc, voi
                : paged_v2_tc<half>(a, workspace, workspace_floats, st);
   return lib ? paged_v1_entry<float>(a, st)
              : paged_v2_tc<float>(a, workspace, workspace_floats, st);
+}
+
+size_t fe_sparse_paged_attention_scratch_ints(int S, int Hkv, int maxb, int num_pages) {
+  if (S < 0 || Hkv < 1 || maxb < 1 || num_pages < 1) return 0;
+  const size_t rows = static_cast<size_t>(S) * Hkv;
+  return rows * (num_pages + size_t{1}) +
+         (fe::step::sparse_two_pass(maxb) ? rows * static_cast<size_t>(maxb) : 0);
 }
 
 size_t fe_paged_attention_v2_workspace_floats(int H, int Hkv, int d, int bs) {

@@ -1,4 +1,4 @@
-// int8 boxes of the keys of full cache pages, the summary that page_select.cu scores.
+// int8 boxes of the keys of full cache pages, the summary that sparse_decode.cu scores.
 //
 // For page b, KV head h and channel c let hi = max_t k[t, c], lo = min_t k[t, c] over the
 // page's block_size tokens, amax = max |k|, and e the smallest exponent with

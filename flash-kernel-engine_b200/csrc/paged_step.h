@@ -1,6 +1,6 @@
 // Internal interface of the serving-step kernels around the paged decode: the step plan
 // (paged_plan.cu), the QKV append (qkv_append.cu), the page boxes (page_bounds.cu) and the
-// page selection of the sparse decode (page_select.cu). Element types are numbered as in
+// sparse decode (sparse_decode.cu). Element types are numbered as in
 // paged_decode.h (DecodeType), cache layouts as KvLayout.
 #pragma once
 
@@ -63,6 +63,9 @@ cudaError_t launch_page_bounds(const BoundsParams& p, int head_dim, int block_si
 
 struct SelectParams {
   const void* q;             // [S, H, d]
+  const void* k_cache;
+  const void* v_cache;
+  void* out;                 // [S, H, d]
   const signed char* values;
   const float* scales;
   const int* block_tables;   // [S, width]
@@ -70,15 +73,19 @@ struct SelectParams {
   int* selected;             // [S, Hkv, num_pages] page indices, ascending, -1 past the count
   int* sel_blocks;           // [S * Hkv, num_pages] block * Hkv + head of each chosen page
   int* sel_lens;             // [S * Hkv] tokens in the chosen pages
+  unsigned* keys;            // [S * Hkv, width] of tables scored in a launch of their own, or null
   int num_seqs, heads, kv_heads, width, num_blocks, block_size;
   int num_pages, keep_first, keep_last;
+  int pieces;                // CTAs a row of that launch (set by the launch)
+  float scale_log2;
   unsigned* err;
 };
-constexpr int kMaxSelectCtas = 16;  // of one (sequence, KV head)
-// Whether page tables of this width fit the kernel's shared memory.
-bool select_width_ok(long long width, int group, int head_dim);
-cudaError_t launch_page_select(const SelectParams& p, int head_dim, int dtype,
-                               cudaStream_t stream);
+// Whether tables of this width are scored in a launch of their own (p.keys).
+bool sparse_two_pass(int width);
+// Whether launch_sparse(fused = true) runs the attention too; otherwise it fills sel_blocks
+// and sel_lens for the paged decode.
+bool sparse_fused(const SelectParams& p, int dtype, int kv_layout);
+cudaError_t launch_sparse(SelectParams p, int head_dim, int dtype, bool fused, cudaStream_t stream);
 
 }  // namespace step
 }  // namespace fe

@@ -73,6 +73,7 @@ _SIGS = {
     "fe_update_page_bounds": ([_P] * 4 + [_I] * 7 + [_P], _I),
     "fe_sparse_paged_attention": ([_P] * 10 + [_I] * 10 + [_F, _I, _I, _P, ctypes.c_size_t, _P],
                                   _I),
+    "fe_sparse_paged_attention_scratch_ints": ([_I] * 4, ctypes.c_size_t),
     "fe_graph_capture": ([None, _P, _P, ctypes.POINTER(ctypes.c_void_p)], _I),
     "fe_graph_launch": ([_P, _P], _I),
     "fe_graph_destroy": ([_P], None),

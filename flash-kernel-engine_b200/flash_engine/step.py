@@ -27,6 +27,7 @@ _plan = _lib.lib.fe_plan_paged_step
 _append = _lib.lib.fe_paged_qkv_append
 _bounds = _lib.lib.fe_update_page_bounds
 _sparse = _lib.lib.fe_sparse_paged_attention
+_scratch_ints = _lib.lib.fe_sparse_paged_attention_scratch_ints
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _LAYOUTS = {"flat": 0, "vllm": 1}
@@ -289,7 +290,8 @@ def sparse_paged_attention(query, key_cache, value_cache, page_bounds, block_tab
         raise ValueError("keep_first >= 0, keep_last >= 1 and num_pages >= their sum expected")
     out = _buffer(out, query.shape, query.dtype, query, "out")
     selected = _buffer(selected, (S, Hkv, num_pages), torch.int32, query, "selected")
-    scratch = torch.empty(S * Hkv * (num_pages + 1), dtype=torch.int32, device=query.device)
+    scratch = torch.empty(_scratch_ints(S, Hkv, maxb, num_pages), dtype=torch.int32,
+                          device=query.device)
     ws, n = _workspace(query, H // Hkv, 1, d, block_size, workspace)
     with _on(query.device):
         st = _sparse(query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),

@@ -413,6 +413,25 @@ def test_sparse_long(S, Hkv, ctx, num_pages):
     check_sparse(make_sparse(S + ctx, lens, 4 * Hkv, Hkv, 64, 16, BF16), num_pages)
 
 
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_sparse_longest(dt):
+    """More pages than a row's scores fit in shared memory."""
+    p = make_sparse(11, [700001], 4, 1, 64, 16, dt)
+    check_sparse(p, 40)
+
+
+@pytest.mark.parametrize("H,Hkv,d,bs", [(16, 4, 128, 16), (36, 4, 64, 32)])
+def test_sparse_many_rows(H, Hkv, d, bs):
+    g = np.random.default_rng(H)
+    check_sparse(make_sparse(12, g.integers(0, 700, 45), H, Hkv, d, bs, BF16), 5)
+
+
+def test_sparse_many_pages_chosen():
+    """A list longer than the attention's shared memory holds goes through the paged decode."""
+    check_sparse(make_sparse(13, [140000, 90], 2, 1, 64, 16, BF16), 8300)
+    check_sparse(make_sparse(13, [140000, 90], 2, 1, 64, 16, BF16), 8100)
+
+
 @pytest.mark.parametrize("ctx", [900, 40000])
 def test_sparse_ties_go_to_the_lower_page(ctx):
     """Equal scores: a zero query, pages that repeat, and few different scores."""

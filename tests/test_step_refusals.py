@@ -1,7 +1,13 @@
 """What the serving-step operators refuse, before any GPU work: the C entries by status, the
-Python operators by exception (the GPU cases with CUDA tensors of wrong shapes and types)."""
+Python operators by exception (the GPU cases with CUDA tensors of wrong shapes and types).
+
+The C entries are called with addresses that are nobody's: where a GPU is present, a missing
+check would send a kernel there. These run without one, where it shows as another status."""
 import pytest
 import torch
+
+no_gpu = pytest.mark.skipif(torch.cuda.is_available(), reason="calls with invalid addresses")
+AT = 1 << 16  # aligned, not mapped
 
 
 def lib():
@@ -9,20 +15,34 @@ def lib():
     return _lib.lib
 
 
+@no_gpu
 def test_plan_entry_refuses():
-    def call(S=1, maxb=4, nb=8, bs=16, mt=4):
-        return lib().fe_plan_paged_step(*[None] * 11, S, maxb, nb, bs, mt, None)
+    def call(S=1, maxb=4, nb=8, bs=16, mt=4, null=None):
+        p = [AT] * 11
+        if null is not None:
+            p[null] = None
+        return lib().fe_plan_paged_step(*p, S, maxb, nb, bs, mt, None)
+    assert call() not in (0, 1)  # accepted, and no device
+    assert call(null=2) not in (0, 1)  # finished may be NULL
+    for i in (0, 1, 3, 4, 5, 6, 7, 8, 9, 10):
+        assert call(null=i) == 1, i
     for kw in (dict(S=-1), dict(S=16385), dict(maxb=-1), dict(nb=0), dict(nb=2 ** 30), dict(bs=0),
                dict(mt=-1), dict(mt=2 ** 30)):
         assert call(**kw) == 1, kw
 
 
+@no_gpu
 def test_append_entry_refuses():
     def call(stride=1000, eps=1e-6, cos=None, sin=None, rd=64, rmax=8, T=1, H=4, Hkv=1, d=64,
-             bs=16, nb=4, dt=0, lay=0):
-        return lib().fe_paged_qkv_append(None, stride, None, None, None, None, None, None, None, 0,
-                                         eps, cos, sin, rd, rmax, 1, T, H, Hkv, d, bs, nb, dt, lay,
-                                         None)
+             bs=16, nb=4, dt=0, lay=0, null=None):
+        p = [AT] * 6
+        if null is not None:
+            p[null] = None
+        return lib().fe_paged_qkv_append(p[0], stride, *p[1:], None, None, 0, eps, cos, sin, rd,
+                                         rmax, 1, T, H, Hkv, d, bs, nb, dt, lay, None)
+    assert call() not in (0, 1)
+    for i in range(6):
+        assert call(null=i) == 1, i
     for kw in (dict(stride=383), dict(eps=-1.0), dict(eps=float("nan")), dict(cos=16),
                dict(sin=16), dict(cos=16, sin=16, rd=65), dict(cos=16, sin=16, rd=66),
                dict(cos=16, sin=16, rd=0), dict(cos=16, sin=16, rmax=0), dict(T=-1), dict(H=0),
@@ -32,28 +52,43 @@ def test_append_entry_refuses():
     assert call(T=0) == 0
 
 
+@no_gpu
 def test_bounds_entry_refuses():
-    def call(k=0, v=0, T=1, Hkv=1, d=64, bs=16, nb=4, dt=0, lay=0):
-        return lib().fe_update_page_bounds(k, v, None, None, T, Hkv, d, bs, nb, dt, lay, None)
-    for kw in (dict(k=8), dict(v=4), dict(T=-1), dict(Hkv=0), dict(d=96), dict(bs=8), dict(nb=0),
+    def call(k=AT, v=AT, s=AT, slots=AT, T=1, Hkv=1, d=64, bs=16, nb=4, dt=0, lay=0):
+        return lib().fe_update_page_bounds(k, v, s, slots, T, Hkv, d, bs, nb, dt, lay, None)
+    assert call() not in (0, 1)
+    for kw in (dict(k=AT + 8), dict(v=AT + 4), dict(s=AT + 2), dict(k=None), dict(v=None),
+               dict(s=None), dict(slots=None), dict(T=-1), dict(Hkv=0), dict(d=96), dict(bs=8), dict(nb=0),
                dict(dt=3), dict(lay=2), dict(lay=1, bs=32), dict(lay=1, dt=2)):
         assert call(**kw) == 1, kw
     assert call(T=0) == 0
 
 
+@no_gpu
 def test_sparse_entry_refuses():
-    none = (1 << 64) - 1
+    lib_ws = (1 << 64) - 1
 
-    def call(q=0, kc=0, val=0, S=1, H=8, Hkv=2, d=64, bs=16, maxb=8, nb=8, k=4, first=1, last=1,
-             dt=0, lay=0, ws=None, n=none):
-        return lib().fe_sparse_paged_attention(q, kc, kc, None, val, None, None, None, None, 0, S,
-                                               H, Hkv, d, bs, maxb, nb, k, first, last, 0.0, dt,
-                                               lay, ws, n, None)
+    def call(S=1, H=8, Hkv=2, d=64, bs=16, maxb=8, nb=8, k=4, first=1, last=1, dt=0, lay=0,
+             ws=None, n=lib_ws, at=None, to=None):
+        p = [AT] * 10
+        if at is not None:
+            p[at] = to
+        return lib().fe_sparse_paged_attention(*p, S, H, Hkv, d, bs, maxb, nb, k, first, last, 0.0,
+                                               dt, lay, ws, n, None)
+    assert call() not in (0, 1)
+    for i in range(10):
+        assert call(at=i) == 1, i
     for kw in (dict(S=-1), dict(H=7), dict(Hkv=0), dict(d=96), dict(bs=8), dict(maxb=0),
                dict(nb=0), dict(k=1), dict(first=-1), dict(last=0), dict(first=4, last=1),
-               dict(dt=3), dict(lay=2), dict(lay=1, bs=32), dict(lay=1, dt=2), dict(kc=8),
-               dict(val=8), dict(S=2 ** 30), dict(nb=2 ** 30), dict(H=2 * 129), dict(maxb=2 ** 24)):
+               dict(dt=3), dict(lay=2), dict(lay=1, bs=32), dict(lay=1, dt=2),
+               dict(at=1, to=AT + 8), dict(at=2, to=AT + 8), dict(at=4, to=AT + 8),
+               dict(at=5, to=AT + 2), dict(at=0, to=AT + 2), dict(at=0, to=AT + 4, dt=2),
+               dict(S=2 ** 30), dict(nb=2 ** 30), dict(H=2 * 129), dict(n=0), dict(ws=AT, n=5)):
         assert call(**kw) == 1, kw
+    assert call(S=0) == 0
+    scratch = lib().fe_sparse_paged_attention_scratch_ints
+    assert scratch(3, 2, 1024, 9) == 60 and scratch(3, 2, 1025, 9) == 60 + 6 * 1025
+    assert scratch(-1, 2, 8, 9) == scratch(1, 0, 8, 9) == scratch(1, 1, 0, 9) == 0
 
 
 def test_operators_have_no_cpu_fallback():
