@@ -592,9 +592,8 @@ int fe_sparse_paged_attention(const void* q, const void* kc, const void* vc, voi
     return kErr;
   if (!aligned(values, 16) || !aligned(scales, 4)) return kErr;
   const long long rows = static_cast<long long>(S) * Hkv;
-  const bool two = fe::step::sparse_two_pass(maxb);
   if (rows * 8 > INT_MAX || rows * (num_pages + 1LL) > INT_MAX || H / Hkv > 128 ||
-      (two && rows * ((maxb + 255LL) / 256) > INT_MAX))
+      static_cast<long long>(S) * ((maxb + 15LL) / 16) > INT_MAX)
     return kErr;
   // The decode sees every (sequence, KV head) as a sequence of its own with one KV head,
   // and the cache as num_blocks * Hkv blocks of it: a page of one head is contiguous.
@@ -632,7 +631,7 @@ int fe_sparse_paged_attention(const void* q, const void* kc, const void* vc, voi
   sp.selected = selected;
   sp.sel_lens = scratch;
   sp.sel_blocks = scratch + rows;
-  sp.keys = two ? reinterpret_cast<unsigned*>(scratch + rows * (num_pages + 1LL)) : nullptr;
+  sp.keys = reinterpret_cast<unsigned*>(scratch + rows * (num_pages + 1LL));
   sp.num_seqs = S;
   sp.heads = H;
   sp.kv_heads = Hkv;
@@ -661,7 +660,7 @@ size_t fe_sparse_paged_attention_scratch_ints(int S, int Hkv, int maxb, int num_
   if (S < 0 || Hkv < 1 || maxb < 1 || num_pages < 1) return 0;
   const size_t rows = static_cast<size_t>(S) * Hkv;
   return rows * (num_pages + size_t{1}) +
-         (fe::step::sparse_two_pass(maxb) ? rows * static_cast<size_t>(maxb) : 0);
+         static_cast<size_t>(fe::step::sparse_key_ints(static_cast<long long>(rows), maxb));
 }
 
 size_t fe_paged_attention_v2_workspace_floats(int H, int Hkv, int d, int bs) {

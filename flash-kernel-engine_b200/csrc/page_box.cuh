@@ -14,12 +14,14 @@ __device__ __forceinline__ bool is_finite(float x) {
 // 2^e for -126 <= e <= 127.
 __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((e + 127) << 23); }
 
-// The smallest e >= kMinBoxExp with amax <= 127 * 2^e, amax finite and >= 0.
+// The smallest e >= kMinBoxExp with amax <= 127 * 2^e, amax finite and >= 0; -7 for 0.
+// amax = m 2^E with m in [0.5, 1): e = E - 7, and one more where m > 127 / 128, that is where
+// the 23 bits below the leading one pass 0x7e0000.
 __device__ __forceinline__ int box_exponent(float amax) {
-  int e;
-  const float m = frexpf(amax, &e);  // amax = m 2^e, m in [0.5, 1), or 0 = 0 2^0
-  e = e - 7 + (m > 127.f / 128.f ? 1 : 0);
-  return e < kMinBoxExp ? kMinBoxExp : e;
+  const unsigned u = __float_as_uint(amax);
+  if (u == 0) return -7;
+  const int e = static_cast<int>(u >> 23) - 126 - 7 + ((u & 0x7fffffu) > 0x7e0000u ? 1 : 0);
+  return e < kMinBoxExp ? kMinBoxExp : e;  // subnormal ones too
 }
 
 }  // namespace step

@@ -73,15 +73,16 @@ struct SelectParams {
   int* selected;             // [S, Hkv, num_pages] page indices, ascending, -1 past the count
   int* sel_blocks;           // [S * Hkv, num_pages] block * Hkv + head of each chosen page
   int* sel_lens;             // [S * Hkv] tokens in the chosen pages
-  unsigned* keys;            // [S * Hkv, width] of tables scored in a launch of their own, or null
+  unsigned* keys;            // sparse_key_ints(...) of scratch
+  unsigned* maxima;          // maxima and key_stride: set by the launch
+  long long key_stride;
   int num_seqs, heads, kv_heads, width, num_blocks, block_size;
   int num_pages, keep_first, keep_last;
-  int pieces;                // CTAs a row of that launch (set by the launch)
   float scale_log2;
   unsigned* err;
 };
-// Whether tables of this width are scored in a launch of their own (p.keys).
-bool sparse_two_pass(int width);
+// Ints of scratch for the scores.
+long long sparse_key_ints(long long rows, int width);
 // Whether launch_sparse(fused = true) runs the attention too; otherwise it fills sel_blocks
 // and sel_lens for the paged decode.
 bool sparse_fused(const SelectParams& p, int dtype, int kv_layout);

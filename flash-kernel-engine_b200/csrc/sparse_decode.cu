@@ -17,17 +17,21 @@
 // in fp32; the weights are rounded to the element type for the product with V, as in
 // paged_decode.cu.
 //
-// One launch where the block tables are at most kOnePassPages wide: a cluster of CTAs
-// serves one (sequence, KV head). Each scores a share of the pages and stores the keys
-// (scores as ordered 32-bit words) into the shared memory of all; each then finds the
-// threshold by itself from histograms of its copy, lists the chosen pages, attends to its
-// share of them, and the partial (m, l, O) are joined over distributed shared memory.
-// Wider tables take a launch of their own for the scores, cut into 256-page pieces whatever
-// the lengths of the sequences, with the keys in global memory.
+// Choice. A score is kept as an ordered 32-bit key, with the largest key of every 8 pages.
+// The m-th largest of those maxima is a lower bound of the m-th largest key, so that only
+// groups that reach it are looked at again (where there are at least 2 m groups): a few
+// hundred of thousands. The threshold then comes from histograms of their keys, refined
+// until the wanted count ends at a bin's edge or a bin is a single key.
 //
-// fp32 caches, the x-packed layout and groups of more than 16 heads take the same
-// selection, which then writes a block table for each (sequence, KV head) that
-// paged_decode.cu runs over.
+// Two launches. page_score_kernel reads the boxes: one CTA an SM takes an equal share of all
+// sequences' 16-page tiles, whatever their lengths, and all KV heads of a tile at once, whose
+// boxes are neighbours in memory. sparse_decode_kernel gives each (sequence, KV head) a
+// cluster of CTAs: each finds the threshold by itself, lists the chosen pages, attends to
+// its share of them, and the partial (m, l, O) are joined over distributed shared memory.
+//
+// fp32 caches, the x-packed layout and groups of more than 16 heads take the same scores and
+// choice, which then writes a block table for each (sequence, KV head) that paged_decode.cu
+// runs over.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -53,10 +57,14 @@ constexpr int kBins = 1 << kBinBits;
 constexpr unsigned kForced = 0xffffffffu;  // key of an always-chosen page, above every score
 constexpr float kInf = __builtin_huge_valf();
 constexpr int kMaxCtas = 8;            // of one (sequence, KV head)
-constexpr int kOnePassPages = 1024;    // widest table scored in the attention's launch
-constexpr int kScorePages = 256;       // pages a CTA of the score launch takes
+constexpr int kScoreWarps = 16;        // of a CTA of the score launch
+constexpr int kScoreRing = 150 * 1024; // bytes of boxes of a CTA in flight, at most
+constexpr int kScoreStages = 32;       // and tiles
+constexpr int kScoreSeqs = 4096;       // most sequences of one launch of it
 constexpr int kMaxFusedPages = 8192;   // most chosen pages whose list fits shared memory
-constexpr int kKeysInSmem = 40960;     // more keys of a row stay in global memory
+constexpr int kGroup = 8;              // pages whose largest key is kept
+constexpr int kMaxGroups = 8192;       // more groups of a row stay in global memory
+constexpr int kMaxKeys = 8192;         // keys looked at again that shared memory takes
 
 // Order-preserving map of a float (no NaN, no -0) to 32 bits.
 __device__ __forceinline__ unsigned key_of(float x) {
@@ -93,243 +101,445 @@ __device__ __forceinline__ uint4 ld_once(const void* p) {
                : "l"(p));
   return v;
 }
+__device__ __forceinline__ void named_bar(int id, int nthreads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
+}
 __device__ __forceinline__ void griddep_wait() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
+__device__ __forceinline__ void griddep_launch() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
 
-// The row of one (sequence, KV head).
-struct Row {
-  int seq, kvh, ctx, pages;
+// One sequence: its length within the table's room, pages, and block table.
+struct Seq {
+  int ctx, pages;
   const int* table;
 };
-__device__ __forceinline__ Row row_of(const SelectParams& p, int row) {
-  Row r;
-  r.seq = row / p.kv_heads;
-  r.kvh = row - r.seq * p.kv_heads;
-  r.ctx = max(0, __ldg(p.context_lens + r.seq));
+__device__ __forceinline__ int pages_of(int ctx, int block_size) {
+  return static_cast<int>((static_cast<long long>(ctx) + block_size - 1) / block_size);
+}
+__device__ __forceinline__ Seq seq_of(const SelectParams& p, int seq) {
+  Seq r;
+  r.ctx = max(0, __ldg(p.context_lens + seq));
   const long long room = static_cast<long long>(p.width) * p.block_size;
   if (r.ctx > room) {
     if (threadIdx.x == 0) atomicOr(p.err, kErrBadBlock);
     r.ctx = static_cast<int>(room);
   }
-  r.pages = (r.ctx + p.block_size - 1) / p.block_size;
-  r.table = p.block_tables + static_cast<long long>(r.seq) * p.width;
+  r.pages = pages_of(r.ctx, p.block_size);
+  r.table = p.block_tables + static_cast<long long>(seq) * p.width;
   return r;
 }
 
-// The group's query heads as whole numbers, a warp a head: rows [q+ | q-] of 2 D bytes and
-// scales 2^eq (+inf for a head with a NaN or an infinity, 0 for the padding to 8 heads).
-template <typename T, int D, int NW>
-__device__ __forceinline__ void quantise_query(const SelectParams& p, const Row& r,
-                                               signed char* qrow, float* qscale) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int G = p.heads / p.kv_heads, GP = (G + 7) / 8 * 8;
-  for (int g = warp; g < GP; g += NW) {
-    constexpr int E = D / 32;
-    float x[E], amax = 0.f;
+// A query head as whole numbers, one warp: [q+ | q-] of 2 D bytes, and (mul, add) that make
+// a score of a sum: (2^eq, 0); with a NaN or an infinity (0, +inf); (0, -inf) without a
+// query, the padding to 8 heads.
+template <typename T, int D>
+struct QueryHead {
+  static constexpr int E = D / 32;
+  float x[E];
+  bool real;
+  __device__ __forceinline__ void load(const T* q) {  // nullptr: no query
+    real = q != nullptr;
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      x[i] = real ? static_cast<float>(q[i * 32 + (threadIdx.x & 31)]) : 0.f;
+  }
+  __device__ __forceinline__ void store(signed char* out, float2* scale) const {
+    const int lane = threadIdx.x & 31;
+    if (!real) {
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i)
+        *reinterpret_cast<uint32_t*>(out + (i * 32 + lane) * 4) = 0;
+      if (lane == 0) *scale = make_float2(0.f, -kInf);
+      return;
+    }
+    float amax = 0.f;
     bool fin = true;
-    const T* q = static_cast<const T*>(p.q) +
-                 (static_cast<long long>(r.seq) * p.heads + r.kvh * G + g) * D;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      x[i] = g < G ? static_cast<float>(q[i * 32 + lane]) : 0.f;
       fin = fin && is_finite(x[i]);
       amax = fmaxf(amax, fabsf(x[i]));
     }
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    // non-negative floats are ordered as their bits
+    amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
     fin = __all_sync(0xffffffffu, fin);
     const int e = box_exponent(fin ? amax : 0.f);
     const float inv = exp2_int(-e);
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       const int v = fin ? __float2int_rn(x[i] * inv) : 0;
-      qrow[g * 2 * D + i * 32 + lane] = static_cast<signed char>(max(v, 0));
-      qrow[g * 2 * D + D + i * 32 + lane] = static_cast<signed char>(min(v, 0));
+      out[i * 32 + lane] = static_cast<signed char>(max(v, 0));
+      out[D + i * 32 + lane] = static_cast<signed char>(min(v, 0));
     }
-    if (lane == 0) qscale[g] = g >= G ? 0.f : fin ? exp2_int(e) : kInf;
+    if (lane == 0) *scale = fin ? make_float2(exp2_int(e), 0.f) : make_float2(0.f, kInf);
   }
-}
+};
 
-// Keys of pages [first, first + 32) of a row by one warp, those below `end`: store(page,
-// key). All of the 32 boxes' bytes are in flight at once.
-template <int D, typename Store>
-__device__ __forceinline__ void score_32(const SelectParams& p, const Row& r,
-                                         const signed char* qrow, const float* qscale, int first,
-                                         int end, Store store) {
-  constexpr int QB = 2 * D;    // bytes of a box, and of a head's row
-  constexpr int CH = QB / 64;  // 64-byte pieces that a quad of lanes reads
+// Keys of the 16 pages from `first` on into keys[0..15], 0 past the row's end, and of their
+// two groups of 8 the largest key that is not always chosen into maxima[0..1], one warp.
+// tile: the boxes of one head in shared memory, rows `pitch` bytes apart; an odd number of
+// 64 bytes, so that a quarter warp's 16-byte reads (2 rows x 4 pieces) hit different banks.
+// sc: the scale of page gq + 8 (cq & 1).
+template <int D>
+__device__ __forceinline__ void score_tile(const SelectParams& p, int pages,
+                                           const unsigned char* tile, int pitch, float sc,
+                                           const signed char* qrow, const float2* qscale, int GP,
+                                           int first, unsigned* keys, unsigned* maxima) {
+  constexpr int CH = 2 * D / 64;
   const int lane = threadIdx.x & 31, gq = lane >> 2, cq = lane & 3;
-  const int GP = (p.heads / p.kv_heads + 7) / 8 * 8;
-  int b = 0;
-  if (first + lane < end) {
-    b = __ldg(r.table + first + lane);
-    if (b < 0 || b >= p.num_blocks) b = 0;  // flagged where the page is listed
-  }
-  const long long page = static_cast<long long>(b) * p.kv_heads + r.kvh;
-  const float ks = __ldg(p.scales + page);
-  uint4 a[4][CH];
+  uint4 a[2][CH];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const long long pk = __shfl_sync(0xffffffffu, page, gq + 8 * k);
-    const uint4* v = reinterpret_cast<const uint4*>(p.values + pk * QB) + cq;
+  for (int k = 0; k < 2; ++k)
 #pragma unroll
-    for (int i = 0; i < CH; ++i) a[k][i] = ld_once(v + 4 * i);
-  }
-  float best[4] = {-kInf, -kInf, -kInf, -kInf};
+    for (int i = 0; i < CH; ++i)
+      a[k][i] = *reinterpret_cast<const uint4*>(tile + (gq + 8 * k) * pitch + (cq + 4 * i) * 16);
+  float best[2] = {-kInf, -kInf};
   for (int h0 = 0; h0 < GP; h0 += 8) {
     int acc[2][4] = {};
-    const uint4* qv = reinterpret_cast<const uint4*>(qrow + (h0 + gq) * QB) + cq;
+    const uint4* qv = reinterpret_cast<const uint4*>(qrow + (h0 + gq) * 2 * D) + cq;
     // the k index of both operands is the byte's place in this lane's 16-byte pieces
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const uint4 v = qv[4 * i];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        mma_s8_16832(acc[t], a[2 * t][i].x, a[2 * t + 1][i].x, a[2 * t][i].y, a[2 * t + 1][i].y,
-                     v.x, v.y);
-        mma_s8_16832(acc[t], a[2 * t][i].z, a[2 * t + 1][i].z, a[2 * t][i].w, a[2 * t + 1][i].w,
-                     v.z, v.w);
-      }
+      mma_s8_16832(acc[0], a[0][i].x, a[1][i].x, a[0][i].y, a[1][i].y, v.x, v.y);
+      mma_s8_16832(acc[1], a[0][i].z, a[1][i].z, a[0][i].w, a[1][i].w, v.z, v.w);
     }
+    const float4 ms = *reinterpret_cast<const float4*>(qscale + h0 + 2 * cq);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const float qs = qscale[h0 + 2 * cq + j];
-      if (qs == 0.f) continue;  // past the group's heads
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        best[k] = fmaxf(best[k],
-                        qs == kInf ? qs : static_cast<float>(acc[k >> 1][(k & 1) * 2 + j]) * qs);
+    for (int k = 0; k < 2; ++k) {  // exact: a sum below 2^24 times a power of two, plus 0
+      best[k] = fmaxf(best[k], fmaf(static_cast<float>(acc[0][2 * k] + acc[1][2 * k]), ms.x, ms.y));
+      best[k] = fmaxf(best[k],
+                      fmaf(static_cast<float>(acc[0][2 * k + 1] + acc[1][2 * k + 1]), ms.z, ms.w));
     }
   }
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < 2; ++k) {
     best[k] = fmaxf(best[k], __shfl_xor_sync(0xffffffffu, best[k], 1));
     best[k] = fmaxf(best[k], __shfl_xor_sync(0xffffffffu, best[k], 2));
   }
-  // lane (gq, cq) keeps page gq + 8 cq
-  const float mine = cq == 0 ? best[0] : cq == 1 ? best[1] : cq == 2 ? best[2] : best[3];
-  const float sc = __shfl_sync(0xffffffffu, ks, gq + 8 * cq);
-  const int j = first + gq + 8 * cq;
-  if (j < end) {
-    const bool kept = j < p.keep_first || j >= r.pages - p.keep_last;
-    store(j, kept ? kForced : key_of((sc == kInf ? sc : mine * sc) + 0.f));  // + 0: no -0
-  }
+  // lanes with an even cq have page gq, those with an odd one page gq + 8
+  const int at = gq + 8 * (cq & 1), j = first + at;
+  const float mine = cq & 1 ? best[1] : best[0];
+  unsigned key = key_of((sc == kInf ? sc : mine * sc) + 0.f);  // + 0: no -0
+  const bool in = j < pages, kept = j < p.keep_first || j >= pages - p.keep_last;
+  unsigned open = in && !kept ? key : 0;
+  key = !in ? 0 : kept ? kForced : key;
+  if (cq < 2) keys[at] = key;
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) open = max(open, __shfl_xor_sync(0xffffffffu, open, o));
+  if (lane < 2) maxima[lane] = open;
 }
 
 template <int NTHR>
 struct SelectShared {
   unsigned hist[kBins];
+  unsigned count[2][(NTHR / 32 + 3) / 4 * 4];
   unsigned sums[NTHR / 32], above[NTHR / 32], equal[NTHR / 32];
-  unsigned kmin, kmax;
-  unsigned bin, over, in_bin;  // result of one histogram round
+  unsigned lo, hi;             // ends of the keys in question
+  unsigned bin, over, in_bin;  // result of one histogram
 };
 
-// The threshold of the K best of `n` > K keys, `kept` of them kForced: chosen are the keys
-// above thr and the first `need` equal to it. Histograms of the keys between the smallest
-// and the largest one, refined until the count ends at a bin's edge or a bin is one key.
-template <int NTHR>
-__device__ __forceinline__ void find_threshold(SelectShared<NTHR>& sh, const unsigned* keys, int n,
-                                               unsigned rem, unsigned& thr, unsigned& need) {
+// The shared memory that a choice works in.
+struct Workspace {
+  unsigned* keys;    // [key_cap]
+  unsigned* maxima;  // [group_cap]
+  int* groups;       // [group_cap] groups looked at again
+  int key_cap, group_cap;
+};
+
+// Of the n keys key(i): the bin of [lo, hi] cut into kBins that holds the rem-th largest of
+// those inside. Leaves hist zeroed.
+template <int NTHR, typename Key>
+__device__ __forceinline__ void find_bin(SelectShared<NTHR>& sh, int n, Key key, unsigned lo,
+                                         unsigned hi, int shift, unsigned rem) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int NW = NTHR / 32, BPT = kBins / NTHR;
-  thr = kForced - 1;
-  need = 0;
-  if (rem == 0) return;
+  for (int i = tid; i < n; i += NTHR) {
+    const unsigned k = key(i);
+    if (k >= lo && k <= hi) atomicAdd(&sh.hist[(k - lo) >> shift], 1u);
+  }
+  __syncthreads();
+  // this thread's bins, the highest ones first over the threads
+  unsigned c[BPT], sum = 0;
+  const int b0 = kBins - (tid + 1) * BPT;
+#pragma unroll
+  for (int i = 0; i < BPT; i += 4) {
+    uint4* h = reinterpret_cast<uint4*>(sh.hist + b0 + i);
+    const uint4 v = *h;
+    *h = make_uint4(0, 0, 0, 0);
+    c[i] = v.x;
+    c[i + 1] = v.y;
+    c[i + 2] = v.z;
+    c[i + 3] = v.w;
+    sum += v.x + v.y + v.z + v.w;
+  }
+  unsigned inc = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned v = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += v;
+  }
+  if (lane == 31) sh.sums[warp] = inc;
+  __syncthreads();
+  unsigned over = inc - sum;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) over += w < warp ? sh.sums[w] : 0;
+  if (over < rem && rem <= over + sum) {
+    bool done = false;
+#pragma unroll
+    for (int i = BPT - 1; i >= 0; --i) {
+      if (!done && rem <= over + c[i]) {
+        sh.bin = b0 + i;
+        sh.over = over;
+        sh.in_bin = c[i];
+        done = true;
+      }
+      over += c[i];
+    }
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ int bin_shift(unsigned lo, unsigned hi) {
+  return lo == hi ? 0 : max(0, 32 - __clz(hi - lo) - kBinBits);
+}
+
+// put(place, page) for the K chosen pages of a row of at most NTHR * J pages, in ascending
+// order: warp w holds the keys of pages [32 J w, 32 J (w + 1)) in registers. The K-th
+// largest key is found bit by bit from the top, one barrier a bit; it ends early where a
+// prefix has exactly K keys at or above it.
+template <int NTHR, int J, typename Shared, typename Put>
+__device__ __forceinline__ void choose_in_registers(Shared& sh, const unsigned* gkeys, int pages,
+                                                    int K, Put put) {
+  constexpr int NW = NTHR / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int first = warp * 32 * J + lane;
+  unsigned k[J];
+#pragma unroll
+  for (int j = 0; j < J; ++j) k[j] = first + j * 32 < pages ? __ldcg(gkeys + first + j * 32) : 0;
+  // the sum of a count over the block: counts of round i in row i & 1
+  auto total = [&](unsigned c, int i) {
+    c = __reduce_add_sync(0xffffffffu, c);
+    if constexpr (NW == 1) return c;
+    if (lane == 0) sh.count[i & 1][warp] = c;
+    __syncthreads();
+    unsigned all = 0;
+#pragma unroll
+    for (int w = 0; w < NW; w += 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(&sh.count[i & 1][w]);
+      all += v.x + v.y + v.z + v.w;
+    }
+    return all;
+  };
+  unsigned thr = 0;  // chosen are the keys above thr and the first `need` equal to it
+  int need = -1;
+  for (int bit = 31; bit >= 0; --bit) {
+    const unsigned at = thr | (1u << bit);
+    unsigned c = 0;
+#pragma unroll
+    for (int j = 0; j < J; ++j) c += k[j] >= at;
+    c = total(c, bit);
+    if (c >= static_cast<unsigned>(K)) thr = at;
+    if (c == static_cast<unsigned>(K)) {
+      thr -= 1;
+      need = 0;
+      break;
+    }
+  }
+  unsigned above = 0, equal = 0;
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    above += k[j] > thr;
+    equal += k[j] == thr;
+  }
+  above = __reduce_add_sync(0xffffffffu, above);
+  equal = __reduce_add_sync(0xffffffffu, equal);
+  unsigned a = 0, e = 0;  // in the warps before
+  if constexpr (NW > 1) {
+    if (lane == 0) {
+      sh.above[warp] = above;
+      sh.equal[warp] = equal;
+    }
+    __syncthreads();
+    unsigned all = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      a += w < warp ? sh.above[w] : 0;
+      e += w < warp ? sh.equal[w] : 0;
+      all += sh.above[w];
+    }
+    above = all;
+  }
+  if (need < 0) need = K - static_cast<int>(above);
+  const unsigned below = (1u << lane) - 1;
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const unsigned ma = __ballot_sync(0xffffffffu, k[j] > thr);
+    const unsigned me = __ballot_sync(0xffffffffu, k[j] == thr);
+    const int ea = static_cast<int>(e) + __popc(me & below);  // equal ones before this page
+    if ((ma >> lane & 1) || ((me >> lane & 1) && ea < need))
+      put(static_cast<int>(a) + __popc(ma & below) + min(ea, need), first + j * 32);
+    a += __popc(ma);
+    e += __popc(me);
+  }
+}
+// The same for any row that fits, NTHR * 8 pages: by one warp up to 256 pages, where the
+// barriers would cost more than the longer turns.
+template <int NTHR, typename Put>
+__device__ __forceinline__ void choose_in_registers(SelectShared<NTHR>& sh, const unsigned* gkeys,
+                                                    int pages, int K, Put put) {
+  if (pages <= 256) {
+    if (threadIdx.x >= 32) return;
+    if (pages <= 128) choose_in_registers<32, 4>(sh, gkeys, pages, K, put);
+    else choose_in_registers<32, 8>(sh, gkeys, pages, K, put);
+  } else if (pages <= NTHR * 3) {
+    choose_in_registers<NTHR, 3>(sh, gkeys, pages, K, put);
+  } else {
+    choose_in_registers<NTHR, 8>(sh, gkeys, pages, K, put);
+  }
+}
+
+// put(place, page) for the K chosen pages of a row in ascending order (more than K pages).
+// gkeys, gmaxima: the row's keys and group maxima.
+template <int NTHR, typename Put>
+__device__ __forceinline__ void choose_pages(SelectShared<NTHR>& sh, const SelectParams& p,
+                                             const Seq& r, const Workspace& ws,
+                                             const unsigned* gkeys, const unsigned* gmaxima,
+                                             Put put) {
+  constexpr int NW = NTHR / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int ng = (r.pages + kGroup - 1) / kGroup;
+  unsigned rem = p.num_pages - p.keep_first - p.keep_last;
+  const unsigned below = (1u << lane) - 1;
+  const unsigned* maxima = ws.maxima;
+  const bool fits = ng <= ws.group_cap;
+  if (!fits) maxima = gmaxima;
+
   if (tid == 0) {
-    sh.kmin = kForced;
-    sh.kmax = 0;
+    sh.lo = kForced;
+    sh.hi = 0;
   }
   for (int i = tid; i < kBins; i += NTHR) sh.hist[i] = 0;
   __syncthreads();
+  // ---- the groups to look at again: those whose largest key reaches `from`, and those of
+  // always-chosen pages
   unsigned lo = kForced, hi = 0;
-  for (int i = tid; i < n; i += NTHR) {
-    const unsigned k = keys[i];
-    lo = min(lo, k);
-    if (k != kForced) hi = max(hi, k);
+  for (int i = tid; i < ng; i += NTHR) {
+    const unsigned k = __ldcg(gmaxima + i);
+    if (fits) ws.maxima[i] = k;
+    if (k) lo = min(lo, k);
+    hi = max(hi, k);
   }
   lo = __reduce_min_sync(0xffffffffu, lo);
   hi = __reduce_max_sync(0xffffffffu, hi);
   if (lane == 0) {
-    atomicMin(&sh.kmin, lo);
-    atomicMax(&sh.kmax, hi);
+    atomicMin(&sh.lo, lo);
+    atomicMax(&sh.hi, hi);
   }
   __syncthreads();
-  lo = sh.kmin;
-  hi = sh.kmax;
-  for (;;) {
-    if (lo == hi) {
-      thr = lo;
-      need = rem;
-      return;
+  lo = sh.lo;
+  hi = sh.hi;
+  bool all = true;  // every group
+  unsigned from = 1;
+  const int first_end = (p.keep_first + kGroup - 1) / kGroup;
+  const int last_beg = (r.pages - p.keep_last) / kGroup;
+  // groups [first_end, last_beg) have no always-chosen page
+  if (fits && 2 * static_cast<int>(rem) <= max(0, last_beg - first_end)) {
+    all = false;
+    if (rem > 0) {
+      const int shift = bin_shift(lo, hi);
+      find_bin<NTHR>(sh, ng, [&](int i) { return maxima[i]; }, lo, hi, shift, rem);
+      from = lo + (sh.bin << shift);
+    } else {
+      from = kForced;
     }
-    const int shift = max(0, 32 - __clz(hi - lo) - kBinBits);
-    for (int i = tid; i < n; i += NTHR) {
-      const unsigned k = keys[i];
-      if (k >= lo && k <= hi) atomicAdd(&sh.hist[(k - lo) >> shift], 1u);
-    }
-    __syncthreads();
-    // this thread's bins, the highest ones first over the threads
-    unsigned c[BPT], sum = 0;
-    const int b0 = kBins - (tid + 1) * BPT;
-#pragma unroll
-    for (int i = 0; i < BPT; ++i) {
-      c[i] = sh.hist[b0 + i];
-      sum += c[i];
-      sh.hist[b0 + i] = 0;
-    }
-    unsigned inc = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned v = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += v;
-    }
-    if (lane == 31) sh.sums[warp] = inc;
-    __syncthreads();
-    unsigned over = inc - sum;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) over += w < warp ? sh.sums[w] : 0;
-    if (over < rem && rem <= over + sum) {
-      bool done = false;
-#pragma unroll
-      for (int i = BPT - 1; i >= 0; --i) {
-        if (!done && rem <= over + c[i]) {
-          sh.bin = b0 + i;
-          sh.over = over;
-          sh.in_bin = c[i];
-          done = true;
-        }
-        over += c[i];
-      }
-    }
-    __syncthreads();
-    const unsigned from = lo + (sh.bin << shift);
-    rem -= sh.over;
-    if (sh.in_bin == rem) {  // the whole bin is chosen
-      thr = from - 1;
-      return;
-    }
-    hi = min(hi, from + ((1u << shift) - 1));
-    lo = from;
   }
-}
-
-// put(place, page) for the chosen pages in ascending order; each warp takes a range.
-template <int NTHR, typename Put>
-__device__ __forceinline__ void list_chosen(SelectShared<NTHR>& sh, const unsigned* keys, int n,
-                                            unsigned thr, unsigned need, Put put) {
-  constexpr int NW = NTHR / 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int nv = ng;
+  if (!all) {
+    // their list, each warp over a range of the groups
+    auto wanted = [&](int i) {
+      return maxima[i] >= from || i < first_end || i >= last_beg;
+    };
+    const int span = ((ng + NW - 1) / NW + 31) / 32 * 32;
+    const int wb = min(ng, warp * span), we = min(ng, wb + span);
+    unsigned cnt = 0;
+    for (int i = wb + lane; i < we; i += 32) cnt += wanted(i);
+    cnt = __reduce_add_sync(0xffffffffu, cnt);
+    if (lane == 0) sh.above[warp] = cnt;
+    __syncthreads();
+    unsigned at = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      at += w < warp ? sh.above[w] : 0;
+      total += sh.above[w];
+    }
+    nv = total;
+    for (int i0 = wb; i0 < we; i0 += 32) {
+      const bool ok = i0 + lane < we && wanted(i0 + lane);
+      const unsigned m = __ballot_sync(0xffffffffu, ok);
+      if (ok) ws.groups[at + __popc(m & below)] = i0 + lane;
+      at += __popc(m);
+    }
+    __syncthreads();
+  }
+  // ---- their keys: place i of the list is page page_at(i)
+  const int n = nv * kGroup;
+  auto page_at = [&](int i) { return all ? i : ws.groups[i / kGroup] * kGroup + i % kGroup; };
+  const bool copied = n <= ws.key_cap;
+  if (copied) {
+    for (int i = tid; i < n; i += NTHR) ws.keys[i] = __ldcg(gkeys + page_at(i));
+    __syncthreads();
+  }
+  auto key = [&](int i) {
+    return copied ? ws.keys[i] : __ldcg(gkeys + page_at(i));
+  };
+  // ---- the threshold: chosen are the keys above thr and the first `need` equal to it
+  unsigned thr = kForced - 1, need = 0;
+  if (rem > 0) {
+    if (all) {
+      unsigned k0 = kForced;
+      for (int i = tid; i < n; i += NTHR) {
+        const unsigned k = key(i);
+        if (k) k0 = min(k0, k);
+      }
+      k0 = __reduce_min_sync(0xffffffffu, k0);
+      if (lane == 0) atomicMin(&sh.lo, k0);
+      __syncthreads();
+      lo = sh.lo;
+    } else {
+      lo = from;
+    }
+    for (;;) {
+      if (lo == hi) {
+        thr = lo;
+        need = rem;
+        break;
+      }
+      const int shift = bin_shift(lo, hi);
+      find_bin<NTHR>(sh, n, key, lo, hi, shift, rem);
+      lo += sh.bin << shift;
+      rem -= sh.over;
+      if (sh.in_bin == rem) {  // the whole bin is chosen
+        thr = lo - 1;
+        break;
+      }
+      hi = min(hi, lo + ((1u << shift) - 1));
+    }
+  }
+  // ---- the list, each warp over a range of the keys
   const int span = ((n + NW - 1) / NW + 31) / 32 * 32;
   const int wb = min(n, warp * span), we = min(n, wb + span);
   unsigned na = 0, ne = 0;
   for (int i = wb + lane; i < we; i += 32) {
-    const unsigned k = keys[i];
+    const unsigned k = key(i);
     na += k > thr;
     ne += k == thr;
   }
   na = __reduce_add_sync(0xffffffffu, na);
   ne = __reduce_add_sync(0xffffffffu, ne);
+  __syncthreads();  // sh.above is read
   if (lane == 0) {
     sh.above[warp] = na;
     sh.equal[warp] = ne;
@@ -342,37 +552,227 @@ __device__ __forceinline__ void list_chosen(SelectShared<NTHR>& sh, const unsign
     e += w < warp ? sh.equal[w] : 0;
   }
   if (na == 0 && (ne == 0 || e >= need)) return;  // uniform in the warp
-  const unsigned below = (1u << lane) - 1;
   for (int i0 = wb; i0 < we; i0 += 32) {
     const int i = i0 + lane;
-    const unsigned k = i < we ? keys[i] : 0;
+    const unsigned k = i < we ? key(i) : 0;
     const unsigned ma = __ballot_sync(0xffffffffu, i < we && k > thr);
     const unsigned me = __ballot_sync(0xffffffffu, i < we && k == thr);
     const unsigned ea = e + __popc(me & below);  // equal ones before this page
     if ((ma >> lane & 1) || ((me >> lane & 1) && ea < need))
-      put(static_cast<int>(a + __popc(ma & below) + min(ea, need)), i);
+      put(static_cast<int>(a + __popc(ma & below) + min(ea, need)), page_at(i));
     a += __popc(ma);
     e += __popc(me);
   }
 }
 
 // ---------------------------------------------------------------------------
-// Scores of wide tables: CTA x takes kScorePages pages of row y into p.keys [rows, width].
+// Scores of all pages into p.keys [rows, key_stride] and p.maxima [rows, key_stride / 8].
+// CTA x takes an equal share of the 16-page tiles of all sequences with more than num_pages
+// pages, blockIdx.y a group of KV heads (a power of two). A producer warp copies each
+// block's boxes of all these heads, which are neighbours in memory, with one bulk copy into
+// a ring of tiles; consumer warp w scores head w % head_group of every (16 / head_group)th
+// tile. A tile's place in the ring always belongs to the same consumer warps (`stages` is a
+// multiple of 16 / head_group), so a parity wait cannot be satisfied by an older phase.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) page_score_kernel(const SelectParams p) {
-  extern __shared__ __align__(16) signed char qrow[];
-  const int GP = (p.heads / p.kv_heads + 7) / 8 * 8;
-  float* qscale = reinterpret_cast<float*>(qrow + GP * 2 * D);
+__global__ void __launch_bounds__(32 * (kScoreWarps + 1), 1)
+    page_score_kernel(const SelectParams p, int head_group, int stages) {
+  constexpr int NW = kScoreWarps, NTH = 32 * (NW + 1);
+  extern __shared__ __align__(16) unsigned char dyn[];
+  __shared__ int warp_tot[NW + 1];
+  __shared__ uint64_t full[kScoreStages], empty[kScoreStages];
+  __shared__ int dead;  // a wait ran out
+  const int G = p.heads / p.kv_heads, GP = (G + 7) / 8 * 8;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int pitch = head_group * 2 * D + 64;  // bytes of a page's boxes in the ring
+  unsigned char* ring = dyn;
+  signed char* qrow = reinterpret_cast<signed char*>(dyn + stages * 16 * pitch);
+  // two sequences' query rows
+  float2* qscale = reinterpret_cast<float2*>(qrow + 2 * head_group * GP * 2 * D);
+  int* pre = reinterpret_cast<int*>(qscale + 2 * head_group * GP);  // [S + 1] tiles before
+  const int head0 = blockIdx.y * head_group, nh = min(head_group, p.kv_heads - head0);
+  if (tid == 0) {
+    dead = 0;
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], nh);
+    }
+    fence_mbar_init();
+  }
+  griddep_launch();  // the next kernel's CTAs take the SMs as this one's leave them
   griddep_wait();
-  const Row r = row_of(p, blockIdx.x / p.pieces);
-  const int beg = static_cast<int>(blockIdx.x % p.pieces) * kScorePages;
-  if (r.pages <= p.num_pages || beg >= r.pages) return;
-  quantise_query<T, D, 8>(p, r, qrow, qscale);
-  __syncthreads();
-  const int first = beg + (threadIdx.x >> 5) * 32;
-  if (first >= r.pages) return;
-  unsigned* keys = p.keys + static_cast<long long>(blockIdx.x / p.pieces) * p.width;
-  score_32<D>(p, r, qrow, qscale, first, r.pages, [&](int j, unsigned key) { keys[j] = key; });
+  // prefix sum of the tiles: a contiguous range of sequences a thread
+  {
+    auto count = [&](int i) {
+      const int pages =
+          min(pages_of(max(0, __ldg(p.context_lens + i)), p.block_size), p.width);
+      return pages > p.num_pages ? (pages + 15) / 16 : 0;
+    };
+    const int per = (p.num_seqs + NTH - 1) / NTH;
+    const int b0 = min(p.num_seqs, tid * per), b1 = min(p.num_seqs, b0 + per);
+    int local = 0;
+    for (int i = b0; i < b1; ++i) local += count(i);
+    int inc = local;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    if (lane == 31) warp_tot[warp] = inc;
+    __syncthreads();
+    int run = inc - local, all = 0;
+#pragma unroll
+    for (int w = 0; w <= NW; ++w) {
+      run += w < warp ? warp_tot[w] : 0;
+      all += warp_tot[w];
+    }
+    for (int i = b0; i < b1; ++i) {
+      pre[i] = run;
+      run += count(i);
+    }
+    if (tid == 0) pre[p.num_seqs] = all;
+    __syncthreads();
+  }
+  const int total = pre[p.num_seqs];
+  int at = static_cast<int>(static_cast<long long>(total) * blockIdx.x / gridDim.x);
+  const int stop = static_cast<int>(static_cast<long long>(total) * (blockIdx.x + 1) / gridDim.x);
+  if (at >= stop) return;
+  // the sequence of tile `at`: the last one that starts at or before it
+  int seq = 0, hi = p.num_seqs;
+  while (hi - seq > 1) {
+    const int mid = (seq + hi) >> 1;
+    if (pre[mid] <= at) seq = mid; else hi = mid;
+  }
+  // block of a page (0 for one out of range: it is flagged where the page is listed)
+  auto block_of = [&](const Seq& r, int j) {
+    int b = 0;
+    if (j < r.pages) {
+      b = __ldg(r.table + j);
+      if (b < 0 || b >= p.num_blocks) b = 0;
+    }
+    return b;
+  };
+  int slot = 0, phase = 0;  // of tile `at`
+
+  if (warp == NW) {
+    // ---- producer: two tiles a step, lanes 0..15 the first one's pages, the others the next
+    const uint64_t policy = l2_policy_evict_first();
+    const uint32_t bytes = nh * 2 * D;
+    while (at < stop) {
+      while (pre[seq + 1] <= at) ++seq;
+      const int t0 = at - pre[seq], t1 = min(stop, pre[seq + 1]) - pre[seq];
+      const Seq r = seq_of(p, seq);
+      auto blocks = [&](int t) { return t < t1 ? block_of(r, t * 16 + lane) : 0; };
+      int b0 = blocks(t0), b1 = blocks(t0 + 2), b2 = blocks(t0 + 4);
+      for (int t = t0; t < t1; t += 2) {
+        const signed char* src =
+            p.values + (static_cast<long long>(b0) * p.kv_heads + head0) * (2 * D);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          if (t + k >= t1) break;
+          const bool free_ =
+              __all_sync(0xffffffffu, mbar_wait(&empty[slot], (phase & 1) ^ 1));
+          if (!free_) {
+            if (lane == 0) atomicOr(p.err, kErrWaitTimeout);
+            return;  // the consumers' waits run out too, after the copies in flight
+          }
+          if (lane == 0) mbar_arrive_expect_tx(&full[slot], 16 * bytes);
+          __syncwarp();
+          if (lane >> 4 == k)
+            bulk_load(ring + (slot * 16 + (lane & 15)) * pitch, src, bytes, &full[slot], policy);
+          if (++slot == stages) {
+            slot = 0;
+            ++phase;
+          }
+        }
+        b0 = b1;
+        b1 = b2;
+        b2 = blocks(t + 6);
+      }
+      at += t1 - t0;
+    }
+    return;
+  }
+
+  // ---- consumers
+  const int head = warp % head_group, group = warp / head_group, step = NW / head_group;
+  const int gq = lane >> 2, cq = lane & 3, page_at = gq + 8 * (cq & 1);
+  // the query rows of a sequence into buffer `buf`
+  auto query = [&](int sq, int buf) {
+    const T* q = static_cast<const T*>(p.q) + (static_cast<long long>(sq) * p.heads + head0 * G) * D;
+    auto head_of = [&](int i) {
+      const int h = i / GP, g = i - h * GP;
+      return i < nh * GP && g < G ? q + (h * G + g) * D : nullptr;
+    };
+    signed char* rows = qrow + buf * head_group * GP * 2 * D;
+    float2* scales = qscale + buf * head_group * GP;
+    for (int i = warp; i < nh * GP; i += 4 * NW) {
+      QueryHead<T, D> qh[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) qh[k].load(head_of(i + k * NW));
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (i + k * NW < nh * GP) qh[k].store(rows + (i + k * NW) * 2 * D, scales + i + k * NW);
+    }
+  };
+  int buf = 0;
+  while (pre[seq + 1] <= at) ++seq;
+  query(seq, 0);
+  while (at < stop) {
+    while (pre[seq + 1] <= at) ++seq;
+    const int t0 = at - pre[seq], t1 = min(stop, pre[seq + 1]) - pre[seq];
+    const Seq r = seq_of(p, seq);
+    // this warp's first tile: its ring places are those with slot % step == group
+    const int skip = (group - slot % step + step) % step;
+    const int end = head < nh ? t1 : 0;
+    auto block_at = [&](int t) { return t < end ? block_of(r, t * 16 + page_at) : 0; };
+    auto scale_of = [&](int b) {
+      return __ldg(p.scales + static_cast<long long>(b) * p.kv_heads + head0 + min(head, nh - 1));
+    };
+    int b1 = block_at(t0 + skip), b2 = block_at(t0 + skip + step);
+    float sc = scale_of(b1);
+    named_bar(1, NW * 32);  // this sequence's query rows are there
+    const signed char* qr = qrow + (buf * head_group + head) * GP * 2 * D;
+    const float2* qs = qscale + (buf * head_group + head) * GP;
+    buf ^= 1;
+    const long long row = static_cast<long long>(seq) * p.kv_heads + head0 + head;
+    unsigned* keys = p.keys + row * p.key_stride;
+    unsigned* maxima = p.maxima + row * (p.key_stride / kGroup);
+    int s = slot + skip, ph = phase;
+    if (s >= stages) {
+      s -= stages;
+      ++ph;
+    }
+    for (int t = t0 + skip; t < end; t += step) {
+      const float sc_next = scale_of(b2);
+      b2 = block_at(t + 2 * step);
+      const bool ok = __all_sync(
+          0xffffffffu, *static_cast<volatile int*>(&dead) == 0 && mbar_wait(&full[s], ph & 1));
+      if (!ok && lane == 0) {
+        dead = 1;
+        atomicOr(p.err, kErrWaitTimeout);
+      }
+      if (ok) {
+        score_tile<D>(p, r.pages, ring + s * 16 * pitch + head * 2 * D, pitch, sc,
+                      qr, qs, GP, t * 16, keys + t * 16, maxima + t * 2);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[s]);
+      }
+      sc = sc_next;
+      s += step;
+      if (s >= stages) {
+        s -= stages;
+        ++ph;
+      }
+    }
+    const int n = slot + t1 - t0;
+    slot = n % stages;
+    phase += n / stages;
+    at += t1 - t0;
+    if (at < stop) {  // the next one's into the other buffer, read before the last barrier
+      while (pre[seq + 1] <= at) ++seq;
+      query(seq, buf);
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -532,66 +932,69 @@ struct WarpAttention {
   }
 };
 
+// The factor of a part (m, l, O) in a join with maximum M. A part without tokens has m = -inf
+// and l = 0; one whose scores are all -inf or NaN keeps its own NaN.
+__device__ __forceinline__ float join_weight(float m, float l, float M) {
+  return m == -kInf ? (l != 0.f ? 1.f : 0.f) : ex2(m - M);
+}
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
+
 // Bytes of the region that holds first the keys, then the warps' partial results.
 template <int D, int NT, int NTHR>
 constexpr int merge_bytes() {
   return NTHR / 32 * 8 * NT * (D + 4 + 2) * 4;
 }
 
+// Byte offsets of the fused kernel's shared memory; the first region holds the keys, group
+// maxima and lists of the choice, and then the warps' partial results.
+struct SparseSmem {
+  int key_cap, group_cap, chosen, got, total;
+};
+
 // Selection and attention of one (sequence, KV head) by a cluster of `ctas` CTAs.
-// key_cap: keys that fit shared memory (0: none are needed there).
 template <typename T, int D, int NT, int NTHR>
-__global__ void __launch_bounds__(NTHR, NTHR == 256 && NT == 1 ? 2 : 1)
-    sparse_decode_kernel(const SelectParams p, int ctas,
-                         int key_cap, int region) {
+__global__ void __launch_bounds__(NTHR, NT == 2 ? 1 : 512 / NTHR) sparse_decode_kernel(const SelectParams p, int ctas, const SparseSmem lay) {
   constexpr int NW = NTHR / 32, HP = 8 * NT;
   extern __shared__ __align__(16) unsigned char dyn[];
-  __shared__ SelectShared<NTHR> sh;
-  __shared__ float part_m[HP], part_l[HP];  // this CTA's joined (m, l)
-  unsigned* keys_s = reinterpret_cast<unsigned*>(dyn);
-  int* chosen = reinterpret_cast<int*>(dyn + region);             // [num_pages]
-  signed char* qrow = reinterpret_cast<signed char*>(chosen + (p.num_pages + 3) / 4 * 4);
-  float* qscale = reinterpret_cast<float*>(qrow + HP * 2 * D);
+  __shared__ __align__(16) SelectShared<NTHR> sh;
+  Workspace ws;
+  ws.keys = reinterpret_cast<unsigned*>(dyn);
+  ws.maxima = ws.keys + lay.key_cap;
+  ws.groups = reinterpret_cast<int*>(ws.maxima + lay.group_cap);
+  ws.key_cap = lay.key_cap;
+  ws.group_cap = lay.group_cap;
+  int* chosen = reinterpret_cast<int*>(dyn + lay.chosen);  // [num_pages]
+  float* got_m = reinterpret_cast<float*>(dyn + lay.got);  // [ctas][HP] of every CTA
+  float* got_l = got_m + ctas * HP;
+  float* got_o = got_l + ctas * HP;  // [ctas][share] of this CTA's share of the output
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, warp = tid >> 5;
   const int row = blockIdx.x / ctas, rank = blockIdx.x % ctas;
+  const int seq = row / p.kv_heads, kvh = row - seq * p.kv_heads;
   const int G = p.heads / p.kv_heads, K = p.num_pages;
+  if (ctas > 1) cluster_arrive();  // waited for before the first store to another CTA
   griddep_wait();
-  const Row r = row_of(p, row);
+  const Seq r = seq_of(p, seq);
   const int P = r.pages, n = min(P, K);
   int* sel = p.selected + static_cast<long long>(row) * K;
 
   // ---- the chosen pages, in every CTA's shared memory
   if (P > K) {
-    const unsigned* keys = keys_s;
-    if (p.keys) {  // scored by page_score_kernel
-      const unsigned* g = p.keys + static_cast<long long>(row) * p.width;
-      if (P <= key_cap) {
-        for (int i = tid; i < P; i += NTHR) keys_s[i] = __ldcg(g + i);
-        __syncthreads();
-      } else {
-        keys = g;
-      }
-    } else {
-      quantise_query<T, D, NW>(p, r, qrow, qscale);
-      if (ctas > 1) cluster.sync(); else __syncthreads();  // all CTAs run: they are stored to
-      for (int first = (rank * NW + warp) * 32; first < P; first += ctas * NW * 32) {
-        score_32<D>(p, r, qrow, qscale, first, P, [&](int j, unsigned key) {
-          if (ctas == 1) {
-            keys_s[j] = key;
-          } else {
-            for (int c = 0; c < ctas; ++c) cluster.map_shared_rank(keys_s, c)[j] = key;
-          }
-        });
-      }
-      if (ctas > 1) cluster.sync(); else __syncthreads();
-    }
-    unsigned thr, need;
-    find_threshold<NTHR>(sh, keys, P, K - p.keep_first - p.keep_last, thr, need);
-    list_chosen<NTHR>(sh, keys, P, thr, need, [&](int at, int page) {
+    auto put = [&](int at, int page) {
       chosen[at] = page;
       if (rank == 0) sel[at] = page;
-    });
+    };
+    const unsigned* keys = p.keys + row * p.key_stride;
+    if (P <= NTHR * 8) {
+      choose_in_registers<NTHR>(sh, keys, P, K, put);
+    } else {
+      choose_pages<NTHR>(sh, p, r, ws, keys, p.maxima + row * (p.key_stride / kGroup), put);
+    }
   } else {
     for (int i = tid; i < K; i += NTHR) {
       if (i < P) chosen[i] = i;
@@ -600,7 +1003,7 @@ __global__ void __launch_bounds__(NTHR, NTHR == 256 && NT == 1 ? 2 : 1)
   }
   __syncthreads();
 
-  // ---- this CTA's share of them: block << 32 is not needed, the list becomes (page, block)
+  // ---- this CTA's share of them
   const int beg = static_cast<int>(static_cast<long long>(n) * rank / ctas);
   const int end = static_cast<int>(static_cast<long long>(n) * (rank + 1) / ctas);
   const int spp = p.block_size / 16, pieces = (end - beg) * spp;
@@ -618,10 +1021,10 @@ __global__ void __launch_bounds__(NTHR, NTHR == 256 && NT == 1 ? 2 : 1)
       at = 0;
       return;
     }
-    at = ((static_cast<long long>(b) * p.kv_heads + r.kvh) * p.block_size + half_ * 16) * D;
+    at = ((static_cast<long long>(b) * p.kv_heads + kvh) * p.block_size + half_ * 16) * D;
   };
   WarpAttention<T, D, NT> w;
-  w.init(static_cast<const T*>(p.q) + (static_cast<long long>(r.seq) * p.heads + r.kvh * G) * D, G);
+  w.init(static_cast<const T*>(p.q) + (static_cast<long long>(seq) * p.heads + kvh * G) * D, G);
   {
     long long at = 0, at_next = 0;
     int limit = 0, limit_next = 0;
@@ -657,7 +1060,9 @@ __global__ void __launch_bounds__(NTHR, NTHR == 256 && NT == 1 ? 2 : 1)
   w.store(om + warp * HP, ol + warp * HP, oo + warp * HP * (D + 4));
   __syncthreads();
   T* out = static_cast<T*>(p.out) +
-           (static_cast<long long>(r.seq) * p.heads + r.kvh * G) * D;
+           (static_cast<long long>(seq) * p.heads + kvh * G) * D;
+  const int share = (G * D + ctas - 1) / ctas;
+  if (ctas > 1) cluster_wait();  // every CTA runs: its shared memory takes stores
   for (int i = tid; i < G * D; i += NTHR) {
     const int h = i / D, d = i - h * D;
     float M = -kInf, L = 0.f, O = 0.f;
@@ -665,101 +1070,92 @@ __global__ void __launch_bounds__(NTHR, NTHR == 256 && NT == 1 ? 2 : 1)
     for (int x = 0; x < NW; ++x) M = fmaxf(M, om[x * HP + h]);
 #pragma unroll
     for (int x = 0; x < NW; ++x) {
-      const float mx = om[x * HP + h];
-      const float f = mx == -kInf ? (ol[x * HP + h] != 0.f ? 1.f : 0.f) : ex2(mx - M);
+      const float f = join_weight(om[x * HP + h], ol[x * HP + h], M);
       L += ol[x * HP + h] * f;
       O += oo[(x * HP + h) * (D + 4) + d] * f;
     }
     if (ctas == 1) {
       out[i] = static_cast<T>(n > 0 ? O / L : 0.f);
     } else {
-      oo[h * (D + 4) + d] = O;  // only this thread reads column d of any warp's row h
-      if (d == 0) {
-        part_m[h] = M;
-        part_l[h] = L;
+      const int to = i / share;
+      cluster.map_shared_rank(got_o, to)[rank * share + i - to * share] = O;
+      if (d < ctas) {
+        cluster.map_shared_rank(got_m, d)[rank * HP + h] = M;
+        cluster.map_shared_rank(got_l, d)[rank * HP + h] = L;
       }
     }
   }
   if (ctas == 1) return;
-  cluster.sync();
-  for (int i = rank * NTHR + tid; i < G * D; i += ctas * NTHR) {
-    const int h = i / D, d = i - h * D;
-    float M = -kInf, mm[kMaxCtas], ll[kMaxCtas], o[kMaxCtas];
-#pragma unroll
-    for (int c = 0; c < kMaxCtas; ++c) {
-      mm[c] = -kInf;
-      ll[c] = o[c] = 0.f;
-      if (c < ctas) {
-        mm[c] = *cluster.map_shared_rank(&part_m[h], c);
-        ll[c] = *cluster.map_shared_rank(&part_l[h], c);
-        o[c] = *cluster.map_shared_rank(&oo[h * (D + 4) + d], c);
-      }
-      M = fmaxf(M, mm[c]);
-    }
-    float L = 0.f, O = 0.f;
-#pragma unroll
-    for (int c = 0; c < kMaxCtas; ++c) {
-      const float f = mm[c] == -kInf ? (ll[c] != 0.f ? 1.f : 0.f) : ex2(mm[c] - M);
-      L += ll[c] * f;
-      O += o[c] * f;
+  cluster.sync();  // all stores to this CTA have arrived, and nothing else will
+  for (int k = tid; k < share && rank * share + k < G * D; k += NTHR) {
+    const int i = rank * share + k, h = i / D;
+    float M = -kInf, L = 0.f, O = 0.f;
+    for (int c = 0; c < ctas; ++c) M = fmaxf(M, got_m[c * HP + h]);
+    for (int c = 0; c < ctas; ++c) {
+      const float f = join_weight(got_m[c * HP + h], got_l[c * HP + h], M);
+      L += got_l[c * HP + h] * f;
+      O += got_o[c * share + k] * f;
     }
     out[i] = static_cast<T>(n > 0 ? O / L : 0.f);
   }
-  cluster.sync();  // no CTA leaves while another reads its shared memory
 }
 
 // ---------------------------------------------------------------------------
 // Selection alone, a CTA a row: the block table (block * Hkv + head) and the length that
 // paged_decode.cu runs over.
-template <typename T, int D, int NTHR>
-__global__ void __launch_bounds__(NTHR) page_select_kernel(const SelectParams p, int key_cap) {
-  constexpr int NW = NTHR / 32;
+template <int NTHR>
+__global__ void __launch_bounds__(NTHR) page_select_kernel(const SelectParams p,
+                                                           const SparseSmem lay) {
   extern __shared__ __align__(16) unsigned char dyn[];
-  __shared__ SelectShared<NTHR> sh;
-  unsigned* keys_s = reinterpret_cast<unsigned*>(dyn);
-  signed char* qrow = reinterpret_cast<signed char*>(keys_s + key_cap);
-  const int GP = (p.heads / p.kv_heads + 7) / 8 * 8;
-  float* qscale = reinterpret_cast<float*>(qrow + GP * 2 * D);
-  const int tid = threadIdx.x, warp = tid >> 5, row = blockIdx.x, K = p.num_pages;
+  const int tid = threadIdx.x, row = blockIdx.x, K = p.num_pages;
+  const int seq = row / p.kv_heads, kvh = row - seq * p.kv_heads;
   griddep_wait();
-  const Row r = row_of(p, row);
+  const Seq r = seq_of(p, seq);
   int* sel = p.selected + static_cast<long long>(row) * K;
   int* blocks = p.sel_blocks + static_cast<long long>(row) * K;
-  auto put = [&](int at, int page) {
-    sel[at] = page;
+  auto block = [&](int page) {
     const int b = __ldg(r.table + page);
     const bool ok = b >= 0 && b < p.num_blocks;
     if (!ok) atomicOr(p.err, kErrBadBlock);
-    blocks[at] = ok ? b * p.kv_heads + r.kvh : -1;
+    return ok ? b * p.kv_heads + kvh : -1;
   };
   const int P = r.pages;
   if (tid == 0)
     p.sel_lens[row] = P <= K ? r.ctx : (K - 1) * p.block_size + r.ctx - (P - 1) * p.block_size;
   if (P <= K) {
     for (int i = tid; i < K; i += NTHR) {
-      if (i < P) put(i, i); else sel[i] = -1;
+      sel[i] = i < P ? i : -1;
+      if (i < P) blocks[i] = block(i);
     }
     return;
   }
-  const unsigned* keys = keys_s;
-  if (p.keys) {
-    keys = p.keys + static_cast<long long>(row) * p.width;
+  auto put = [&](int at, int page) { sel[at] = page; };
+  const unsigned* keys = p.keys + row * p.key_stride;
+  __shared__ __align__(16) SelectShared<NTHR> sh;
+  if (P <= NTHR * 8) {
+    choose_in_registers<NTHR>(sh, keys, P, K, put);
   } else {
-    quantise_query<T, D, NW>(p, r, qrow, qscale);
-    __syncthreads();
-    for (int first = warp * 32; first < P; first += NW * 32)
-      score_32<D>(p, r, qrow, qscale, first, P, [&](int j, unsigned key) { keys_s[j] = key; });
-    __syncthreads();
+    Workspace ws;
+    ws.keys = reinterpret_cast<unsigned*>(dyn);
+    ws.maxima = ws.keys + lay.key_cap;
+    ws.groups = reinterpret_cast<int*>(ws.maxima + lay.group_cap);
+    ws.key_cap = lay.key_cap;
+    ws.group_cap = lay.group_cap;
+    choose_pages<NTHR>(sh, p, r, ws, keys, p.maxima + row * (p.key_stride / kGroup), put);
   }
-  unsigned thr, need;
-  find_threshold<NTHR>(sh, keys, P, K - p.keep_first - p.keep_last, thr, need);
-  list_chosen<NTHR>(sh, keys, P, thr, need, put);
+  __syncthreads();  // the list is written, and read back by its CTA
+#pragma unroll 4
+  for (int i = tid; i < K; i += NTHR) blocks[i] = block(sel[i]);
 }
 
 // ---------------------------------------------------------------------------
 // host launch
 
-bool sparse_two_pass(int width) { return width > kOnePassPages; }
+// Ints of a row's keys (whole 16-page tiles), and of all keys and maxima.
+static long long key_stride(int width) { return (width + 15LL) / 16 * 16; }
+long long sparse_key_ints(long long rows, int width) {
+  return rows * (key_stride(width) + key_stride(width) / kGroup);
+}
 
 bool sparse_fused(const SelectParams& p, int dtype, int kv_layout) {
   return dtype != paged::kF32 && kv_layout == paged::kKvFlat && p.heads / p.kv_heads <= 16 &&
@@ -767,7 +1163,8 @@ bool sparse_fused(const SelectParams& p, int dtype, int kv_layout) {
 }
 
 // Every kernel waits for its predecessor before it reads anything, so they may all be
-// placed while it finishes; none lets its successor start early.
+// placed while it finishes. Only the score kernel lets its successor be placed early, which
+// is one of this file.
 static void launch_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, long long grid,
                           int threads, int smem, int ctas, cudaStream_t st) {
   cfg = cudaLaunchConfig_t{};
@@ -789,69 +1186,99 @@ static void launch_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, lo
 }
 
 template <typename T, int D>
-static cudaError_t launch_scores(SelectParams& p, cudaStream_t st) {
-  const int GP = (p.heads / p.kv_heads + 7) / 8 * 8;
-  const int smem = GP * (2 * D + 4);
-  const cudaError_t e =
-      ensure_smem_optin(reinterpret_cast<const void*>(page_score_kernel<T, D>), smem);
-  if (e != cudaSuccess) return e;
-  p.pieces = (p.width + kScorePages - 1) / kScorePages;
-  cudaLaunchConfig_t cfg;
-  cudaLaunchAttribute attr[2];
-  launch_config(cfg, attr, static_cast<long long>(p.num_seqs) * p.kv_heads * p.pieces, 256, smem, 1,
-                st);
-  return cudaLaunchKernelEx(&cfg, page_score_kernel<T, D>, p);
+static cudaError_t launch_scores(const SelectParams& all, cudaStream_t st) {
+  auto kern = page_score_kernel<T, D>;
+  const int G = all.heads / all.kv_heads, GP = (G + 7) / 8 * 8;
+  // KV heads of a CTA, a power of two: 8 (whose boxes fill 2 KB of memory), fewer where
+  // there are fewer or where their query rows would take more than 16 KB
+  int hg = 8;
+  while (hg > 1 && (hg / 2 >= all.kv_heads || hg * GP * 2 * D > 16384)) hg /= 2;
+  const int groups = (all.kv_heads + hg - 1) / hg;
+  const int pitch = hg * 2 * D + 64, step = kScoreWarps / hg;
+  const int stages = std::min(kScoreStages, kScoreRing / (16 * pitch)) / step * step;
+  for (int s0 = 0; s0 < all.num_seqs; s0 += kScoreSeqs) {
+    SelectParams p = all;
+    p.num_seqs = std::min(kScoreSeqs, all.num_seqs - s0);
+    p.q = static_cast<const T*>(all.q) + static_cast<long long>(s0) * all.heads * D;
+    p.context_lens += s0;
+    p.block_tables += static_cast<long long>(s0) * all.width;
+    p.keys += static_cast<long long>(s0) * all.kv_heads * all.key_stride;
+    p.maxima += static_cast<long long>(s0) * all.kv_heads * (all.key_stride / kGroup);
+    const int smem = stages * 16 * pitch + 2 * hg * GP * (2 * D + 8) + (p.num_seqs + 1) * 4;
+    const cudaError_t e = ensure_smem_optin(reinterpret_cast<const void*>(kern), smem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr[2];
+    launch_config(cfg, attr, std::max(1, sm_count() / groups), 32 * (kScoreWarps + 1), smem, 1,
+                  st);
+    cfg.gridDim.y = groups;
+    const cudaError_t l = cudaLaunchKernelEx(&cfg, kern, p, hg, stages);
+    if (l != cudaSuccess) return l;
+  }
+  return cudaSuccess;
+}
+
+// Shared memory of the choice (and of `partials` bytes in its place afterwards), of the
+// list of chosen pages, and of `got` bytes from the other CTAs.
+static SparseSmem smem_layout(const SelectParams& p, int partials, int list, int got) {
+  SparseSmem l;
+  l.key_cap = static_cast<int>(std::min<long long>(p.key_stride, kMaxKeys));
+  l.group_cap = static_cast<int>(std::min<long long>(p.key_stride / kGroup, kMaxGroups) + 3) / 4 * 4;
+  l.chosen = (std::max((l.key_cap + 2 * l.group_cap) * 4, partials) + 15) / 16 * 16;
+  l.got = l.chosen + (list + 3) / 4 * 16;
+  l.total = l.got + got;
+  return l;
 }
 
 template <typename T, int D, int NT, int NTHR>
 static cudaError_t launch_fused(const SelectParams& p, int ctas, cudaStream_t st) {
   auto kern = sparse_decode_kernel<T, D, NT, NTHR>;
-  const int key_cap = std::min(p.width, kKeysInSmem);
-  const int region = (std::max(key_cap * 4, merge_bytes<D, NT, NTHR>()) + 15) / 16 * 16;
-  const int smem = region + (p.num_pages + 3) / 4 * 16 + 8 * NT * (2 * D + 4);
-  const cudaError_t e = ensure_smem_optin(reinterpret_cast<const void*>(kern), smem);
+  const int share = (p.heads / p.kv_heads * D + ctas - 1) / ctas;
+  const SparseSmem lay = smem_layout(p, merge_bytes<D, NT, NTHR>(), p.num_pages,
+                                     ctas > 1 ? ctas * (share + 16 * NT) * 4 : 0);
+  const cudaError_t e = ensure_smem_optin(reinterpret_cast<const void*>(kern), lay.total);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr[2];
-  launch_config(cfg, attr, static_cast<long long>(p.num_seqs) * p.kv_heads * ctas, NTHR, smem, ctas,
-                st);
-  return cudaLaunchKernelEx(&cfg, kern, p, ctas, key_cap, region);
+  launch_config(cfg, attr, static_cast<long long>(p.num_seqs) * p.kv_heads * ctas, NTHR, lay.total,
+                ctas, st);
+  return cudaLaunchKernelEx(&cfg, kern, p, ctas, lay);
 }
 
-template <typename T, int D>
+template <int NTHR>
 static cudaError_t launch_select(const SelectParams& p, cudaStream_t st) {
-  constexpr int NTHR = 512;
-  auto kern = page_select_kernel<T, D, NTHR>;
-  const int key_cap = p.keys ? 0 : (p.width + 3) / 4 * 4;
-  const int smem = key_cap * 4 + (p.heads / p.kv_heads + 7) / 8 * 8 * (2 * D + 4);
-  const cudaError_t e = ensure_smem_optin(reinterpret_cast<const void*>(kern), smem);
+  auto kern = page_select_kernel<NTHR>;
+  const SparseSmem lay = smem_layout(p, 0, 0, 0);
+  const cudaError_t e = ensure_smem_optin(reinterpret_cast<const void*>(kern), lay.total);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr[2];
-  launch_config(cfg, attr, static_cast<long long>(p.num_seqs) * p.kv_heads, NTHR, smem, 1, st);
-  return cudaLaunchKernelEx(&cfg, kern, p, key_cap);
+  launch_config(cfg, attr, static_cast<long long>(p.num_seqs) * p.kv_heads, NTHR, lay.total, 1, st);
+  return cudaLaunchKernelEx(&cfg, kern, p, lay);
 }
 
 template <typename T, int D>
 static cudaError_t launch_d(SelectParams& p, bool fused, cudaStream_t st) {
-  if (p.keys) {
-    const cudaError_t e = launch_scores<T, D>(p, st);
-    if (e != cudaSuccess) return e;
-  }
+  p.key_stride = key_stride(p.width);
+  p.maxima = p.keys + p.key_stride * p.num_seqs * p.kv_heads;
+  const cudaError_t e = launch_scores<T, D>(p, st);
+  if (e != cudaSuccess) return e;
   if constexpr (!std::is_same<T, float>::value) {
     if (fused) {
-      // CTAs a row: enough to fill the GPU, at least two 16-token pieces a warp's turn each
+      // CTAs a row: enough to fill the GPU, with 4 pieces of 16 tokens each at least
       const long long rows = static_cast<long long>(p.num_seqs) * p.kv_heads;
       int ctas = 1;
       while (ctas < kMaxCtas && rows * ctas * 2 <= sm_count() &&
              p.num_pages * (p.block_size / 16) >= 4 * ctas)
         ctas *= 2;
       if (p.heads / p.kv_heads > 8) return launch_fused<T, D, 2, 256>(p, ctas, st);
-      if (rows * ctas <= sm_count()) return launch_fused<T, D, 1, 512>(p, ctas, st);
-      return launch_fused<T, D, 1, 256>(p, ctas, st);
+      // more rows than SMs: four CTAs of 4 warps an SM, so that one's choice runs beside
+      // the others' copies (batch of 64 mixed contexts: 80 us; 90 us with two of 8 warps)
+      if (rows * ctas > sm_count()) return launch_fused<T, D, 1, 128>(p, ctas, st);
+      return launch_fused<T, D, 1, 512>(p, ctas, st);
     }
   }
-  return launch_select<T, D>(p, st);
+  return launch_select<512>(p, st);
 }
 
 template <typename T>

@@ -458,11 +458,10 @@ int fe_update_page_bounds(const void* k_cache, signed char* values, float* scale
  * kv_layout and the workspace are those of fe_paged_attention_ex; num_blocks must be
  * given, scale is positive. Outputs: out [S, H, d]; selected [S, Hkv, num_pages], the
  * chosen page indices in ascending order, -1 past their count. scratch:
- * fe_sparse_paged_attention_scratch_ints ints, any content. One launch for bf16 / fp16 with
- * the flat layout, at most 16 query heads a KV head and 8192 pages, one more for the scores
- * of tables wider than 1024 pages; otherwise the selection, then the decode of
- * fe_paged_attention_ex with a block table for each (sequence, KV head), which alone uses
- * the workspace. */
+ * fe_sparse_paged_attention_scratch_ints ints, any content. Two launches (scores, attention)
+ * for bf16 / fp16 with the flat layout, at most 16 query heads a KV head and 8192 pages;
+ * otherwise scores, selection and the decode of fe_paged_attention_ex with a block table for
+ * each (sequence, KV head), which alone uses the workspace. */
 size_t fe_sparse_paged_attention_scratch_ints(int num_seqs, int num_kv_heads,
                                               int max_blocks_per_seq, int num_pages);
 int fe_sparse_paged_attention(const void* q, const void* k_cache, const void* v_cache, void* out,

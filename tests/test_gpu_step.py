@@ -399,9 +399,10 @@ def test_sparse_vllm_layout(dt):
 
 
 @pytest.mark.parametrize("first,last,num_pages", [(0, 1, 1), (0, 1, 4), (3, 2, 5), (2, 9, 12),
-                                                  (0, 4, 33)])
-def test_sparse_kept_pages(first, last, num_pages):
-    check_sparse(make_sparse(2, LENS, 8, 2, 64, 16, BF16), num_pages, first, last)
+                                                  (0, 4, 33), (33, 20, 55), (0, 50, 60)])
+@pytest.mark.parametrize("lens", [LENS, [3000, 2999]])
+def test_sparse_kept_pages(first, last, num_pages, lens):
+    check_sparse(make_sparse(2, lens, 8, 2, 64, 16, BF16), num_pages, first, last)
 
 
 @pytest.mark.parametrize("S,Hkv,ctx", [(1, 1, 9001), (2, 1, 70000), (1, 8, 20000), (3, 2, 33333)])

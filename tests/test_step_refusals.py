@@ -87,7 +87,7 @@ def test_sparse_entry_refuses():
         assert call(**kw) == 1, kw
     assert call(S=0) == 0
     scratch = lib().fe_sparse_paged_attention_scratch_ints
-    assert scratch(3, 2, 1024, 9) == 60 and scratch(3, 2, 1025, 9) == 60 + 6 * 1025
+    assert scratch(3, 2, 64, 9) >= 60 + 6 * 64 and scratch(3, 2, 5000, 9) >= 60 + 6 * 5000
     assert scratch(-1, 2, 8, 9) == scratch(1, 0, 8, 9) == scratch(1, 1, 0, 9) == 0
 
 
