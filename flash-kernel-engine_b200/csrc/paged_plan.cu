@@ -12,11 +12,13 @@
 //
 // One launch, no waiting between CTAs: every CTA forms the three prefix sums (tokens,
 // blocks taken, blocks given back) of all requests in its own shared memory (12 bytes a
-// request) and then writes its share of the tokens, 4 consecutive ones a thread. A token
-// takes its block from the ring directly and not from the table, so no CTA reads what
-// another one writes: the ring's popped and pushed ranges are disjoint, and the only table
-// entry a token reads is the request's last, partly filled block. Rows of finished
-// requests are read and rewritten by one thread an entry.
+// request) and then writes its share of the tokens, one a thread. A token takes its block
+// from the ring directly and not from the table, so no CTA reads what another one writes:
+// the ring's popped and pushed ranges are disjoint, and the only table entry a token reads
+// is the request's last, partly filled block. Rows of finished requests are read and
+// rewritten by one thread an entry. What bounds it is latency: the lengths' loads, the
+// sums (all loads first, then a contiguous range of requests a thread and one block-wide
+// scan of the ranges' sums), a binary search a token and the load of its block.
 #include <algorithm>
 
 #include "internal.h"
@@ -43,186 +45,184 @@ __device__ __forceinline__ unsigned warp_scan_sat(unsigned v, int lane) {
   return v;
 }
 
+// Where entry s of a prefix sum lies: one word in 33 is left out, so that threads that walk
+// ranges of 2^k entries side by side hit different banks.
+__device__ __forceinline__ int at(int s) { return s + (s >> 5); }
+__host__ __device__ constexpr int padded(int n) { return n + (n >> 5) + 1; }
+
 // Largest s in [0, S) with cu[s] <= t, for t < cu[S].
-__device__ __forceinline__ int request_of(const int* cu, int S, int t) {
+__device__ __forceinline__ int request_of(const unsigned* cu, int S, unsigned t) {
   int lo = 0, hi = S;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= t) lo = mid; else hi = mid;
+    if (cu[at(mid)] <= t) lo = mid; else hi = mid;
   }
   return lo;
 }
 
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) {
-  extern __shared__ int smem[];
+  extern __shared__ unsigned smem[];
   constexpr int NW = kPlanThreads / 32;
   __shared__ unsigned wsum[3][NW];
   __shared__ int first_fail;
   const int S = p.num_seqs, bs = p.block_size, nb = p.num_blocks;
-  int* cu = smem;            // [S + 1] tokens before request s
-  int* pop = cu + S + 1;     // [S + 1] blocks taken before request s
-  int* push = pop + S + 1;   // [S + 1] blocks given back before request s
+  // [S + 1] each: tokens, blocks taken and blocks given back before request s
+  unsigned* cu = smem;
+  unsigned* pop = cu + padded(S + 1);
+  unsigned* push = pop + padded(S + 1);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int head = max(0, __ldg(p.state)) % nb;
   const int count = min(max(0, __ldg(p.state + 1)), nb);
   const long long room = static_cast<long long>(p.width) * bs;
+  auto finished = [&](int s) { return p.finished && p.finished[s]; };
+  // ring entry head + k, k < 2^30
+  auto ring = [&](unsigned k) -> int& {
+    unsigned i = head + k % nb;
+    if (i >= static_cast<unsigned>(nb)) i -= nb;
+    return p.free_blocks[i];
+  };
   if (tid == 0) {
     first_fail = S;
     cu[0] = pop[0] = push[0] = 0;
   }
+  // what each request asks for, as entry s + 1
+#pragma unroll 4
+  for (int s = tid; s < S; s += kPlanThreads) {
+    const int held = max(0, __ldg(p.context_lens + s)), add = max(0, __ldg(p.new_lens + s));
+    const bool fin = finished(s);
+    const int ctx = fin ? 0 : held;
+    const long long end = static_cast<long long>(ctx) + add;
+    const long long have = (static_cast<long long>(held) + bs - 1) / bs;
+    const long long need = (end + bs - 1) / bs - (fin ? 0 : have);
+    // a request that its row cannot hold asks for more than there is
+    cu[at(s + 1)] = end <= room ? min(add, kMaxPlanCount) : kMaxPlanCount;
+    pop[at(s + 1)] = static_cast<unsigned>(min(need, static_cast<long long>(kMaxPlanCount)));
+    push[at(s + 1)] = fin ? static_cast<unsigned>(min(have, static_cast<long long>(p.width))) : 0;
+  }
   __syncthreads();
-  unsigned run0 = 0, run1 = 0, run2 = 0;  // sums of the tiles so far
-  for (int base = 0; base < S; base += kPlanThreads) {
-    const int s = base + tid;
-    unsigned n = 0, need = 0, give = 0;
-    bool fits = true;
-    if (s < S) {
-      int ctx = max(0, __ldg(p.context_lens + s));
-      const int add = max(0, __ldg(p.new_lens + s));
-      if (p.finished && p.finished[s]) {
-        give = static_cast<unsigned>(min((static_cast<long long>(ctx) + bs - 1) / bs,
-                                         static_cast<long long>(p.width)));
-        ctx = 0;
-      }
-      const long long end = static_cast<long long>(ctx) + add;
-      fits = end <= room;
-      n = min(static_cast<unsigned>(add), static_cast<unsigned>(kMaxPlanCount));
-      need = static_cast<unsigned>(
-          min((end + bs - 1) / bs - (static_cast<long long>(ctx) + bs - 1) / bs,
-              static_cast<long long>(kMaxPlanCount)));
-    }
-    unsigned i0 = warp_scan_sat(n, lane), i1 = warp_scan_sat(need, lane),
-             i2 = warp_scan_sat(give, lane);
-    if (lane == 31) {
-      wsum[0][warp] = i0;
-      wsum[1][warp] = i1;
-      wsum[2][warp] = i2;
-    }
-    __syncthreads();
-    unsigned b0 = run0, b1 = run1, b2 = run2;
+  // prefix sums: this thread's range, then the ranges before it
+  const int per = (S + kPlanThreads - 1) / kPlanThreads;
+  const int s0 = min(S, tid * per), s1 = min(S, s0 + per);
+  unsigned own[3] = {0, 0, 0};
+  for (int s = s0; s < s1; ++s) {
+    own[0] = sat_add(own[0], cu[at(s + 1)]);
+    own[1] = sat_add(own[1], pop[at(s + 1)]);
+    own[2] = sat_add(own[2], push[at(s + 1)]);
+  }
+  unsigned run[3];
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const unsigned w0 = wsum[0][w], w1 = wsum[1][w], w2 = wsum[2][w];
-      if (w < warp) {
-        b0 = sat_add(b0, w0);
-        b1 = sat_add(b1, w1);
-        b2 = sat_add(b2, w2);
-      }
-      run0 = sat_add(run0, w0);
-      run1 = sat_add(run1, w1);
-      run2 = sat_add(run2, w2);
+  for (int k = 0; k < 3; ++k) {
+    const unsigned inc = warp_scan_sat(own[k], lane);
+    if (lane == 31) wsum[k][warp] = inc;
+    const unsigned before = __shfl_up_sync(0xffffffffu, inc, 1);
+    run[k] = lane == 0 ? 0 : before;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    if (w < warp) {
+#pragma unroll
+      for (int k = 0; k < 3; ++k) run[k] = sat_add(run[k], wsum[k][w]);
     }
-    i0 = sat_add(i0, b0);
-    i1 = sat_add(i1, b1);
-    i2 = sat_add(i2, b2);
-    if (s < S) {
-      cu[s + 1] = static_cast<int>(i0);
-      pop[s + 1] = static_cast<int>(i1);
-      push[s + 1] = static_cast<int>(i2);
-      if (!fits || i0 > static_cast<unsigned>(p.max_tokens) || i1 > static_cast<unsigned>(count))
-        atomicMin(&first_fail, s);
-    }
+  }
+  int fail = S;
+  for (int s = s0; s < s1; ++s) {
+    const int i = at(s + 1);
+    cu[i] = run[0] = sat_add(run[0], cu[i]);
+    pop[i] = run[1] = sat_add(run[1], pop[i]);
+    push[i] = run[2] = sat_add(run[2], push[i]);
+    if (run[0] > static_cast<unsigned>(p.max_tokens) || run[1] > static_cast<unsigned>(count))
+      fail = min(fail, s);
+  }
+  if (fail < S) atomicMin(&first_fail, fail);
+  __syncthreads();
+  const int served = first_fail;
+  const unsigned total = cu[at(served)], taken = pop[at(served)];
+  if (served < S) {
+    __syncthreads();
+    for (int s = served + 1 + tid; s <= S; s += kPlanThreads) cu[at(s)] = total;
     __syncthreads();
   }
-  const int served = first_fail;
-  const int total = cu[served];
-  __syncthreads();
-  for (int s = served + 1 + tid; s <= S; s += kPlanThreads) cu[s] = total;
-  __syncthreads();
-  const int taken = pop[served];
 
   const int gtid = blockIdx.x * kPlanThreads + tid, nth = gridDim.x * kPlanThreads;
+  // tokens
+  for (int t = gtid; t < p.max_tokens; t += nth) {
+    int pos = -1;
+    long long slot = -1;
+    if (static_cast<unsigned>(t) < total) {
+      const int s = request_of(cu, S, t);
+      const bool fresh = finished(s);
+      const int ctx = fresh ? 0 : max(0, __ldg(p.context_lens + s));
+      const int have = (ctx + bs - 1) / bs;
+      pos = ctx + t - static_cast<int>(cu[at(s)]);
+      const int j = pos / bs, off = pos - j * bs;
+      int* entry = p.block_tables + static_cast<long long>(s) * p.width + j;
+      int block;
+      if (j < have) {
+        block = *entry;
+      } else {
+        block = ring(pop[at(s)] + (j - have));
+        if (off == 0 && !fresh) *entry = block;
+      }
+      slot = static_cast<long long>(block) * bs + off;
+    }
+    p.positions[t] = pos;
+    p.slots[t] = slot;
+  }
+  // lengths and offsets
   if (gtid == 0) {
-    const long long left = static_cast<long long>(count) - taken + run2;
-    p.state_out[0] = static_cast<int>((static_cast<long long>(head) + taken) % nb);
+    const long long left = static_cast<long long>(count) - taken + push[at(S)];
+    p.state_out[0] = static_cast<int>((static_cast<unsigned>(head) + taken) % nb);
     p.state_out[1] = static_cast<int>(min(left, static_cast<long long>(nb)));
     p.state_out[2] = served;
     p.state_out[3] = total;
     p.cu_seqlens[0] = 0;
-    if (static_cast<long long>(count) + run2 > nb) atomicOr(p.err, kErrBadBlock);
+    if (static_cast<long long>(count) + push[at(S)] > nb) atomicOr(p.err, kErrBadBlock);
   }
   for (int s = gtid; s < S; s += nth) {
-    const int ctx = p.finished && p.finished[s] ? 0 : max(0, __ldg(p.context_lens + s));
-    p.cu_seqlens[s + 1] = cu[s + 1];
-    p.context_lens_out[s] = ctx + cu[s + 1] - cu[s];
+    const unsigned end = cu[at(s + 1)];
+    p.cu_seqlens[s + 1] = end;
+    p.context_lens_out[s] =
+        (finished(s) ? 0 : max(0, __ldg(p.context_lens + s))) + static_cast<int>(end - cu[at(s)]);
   }
   // finished rows, a warp each: entry j goes back to the ring and then takes the row's new
   // block j
   if (p.finished) {
     for (int s = gtid >> 5; s < S; s += nth >> 5) {
       if (!p.finished[s]) continue;
-      const int held = static_cast<int>(
-          min((max(0LL, static_cast<long long>(__ldg(p.context_lens + s))) + bs - 1) / bs,
-              static_cast<long long>(p.width)));
-      const int now = (cu[s + 1] - cu[s] + bs - 1) / bs;
+      const int held = static_cast<int>(push[at(s + 1)] - push[at(s)]);
+      const int now = (static_cast<int>(cu[at(s + 1)] - cu[at(s)]) + bs - 1) / bs;
       int* row = p.block_tables + static_cast<long long>(s) * p.width;
       for (int j = lane; j < max(held, now); j += 32) {
-        const long long to = static_cast<long long>(count) + push[s] + j;
-        if (j < held && to < nb) p.free_blocks[(head + to) % nb] = row[j];
-        if (j < now) row[j] = p.free_blocks[(static_cast<long long>(head) + pop[s] + j) % nb];
-      }
-    }
-  }
-  // tokens, 4 a thread
-  for (long long t0 = 4LL * gtid; t0 < p.max_tokens; t0 += 4LL * nth) {
-    int pos[4];
-    long long slot[4];
-    int s = -1, ctx = 0, have = 0, beg = 0, end = 0;
-    bool fresh = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int t = static_cast<int>(t0) + i;
-      pos[i] = -1;
-      slot[i] = -1;
-      if (t0 + i >= total) continue;
-      if (s < 0 || t >= end) {
-        s = request_of(cu, S, t);
-        beg = cu[s];
-        end = cu[s + 1];
-        fresh = p.finished && p.finished[s];
-        ctx = fresh ? 0 : max(0, __ldg(p.context_lens + s));
-        have = (ctx + bs - 1) / bs;
-      }
-      const int at = ctx + t - beg;
-      const int j = at / bs, off = at - j * bs;
-      int* row = p.block_tables + static_cast<long long>(s) * p.width;
-      int block;
-      if (j < have) {
-        block = row[j];
-      } else {
-        block = p.free_blocks[(static_cast<long long>(head) + pop[s] + (j - have)) % nb];
-        if (off == 0 && !fresh) row[j] = block;
-      }
-      pos[i] = at;
-      slot[i] = static_cast<long long>(block) * bs + off;
-    }
-    if (t0 + 4 <= p.max_tokens && (reinterpret_cast<uintptr_t>(p.positions) & 15) == 0 &&
-        (reinterpret_cast<uintptr_t>(p.slots) & 15) == 0) {
-      *reinterpret_cast<int4*>(p.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
-      *reinterpret_cast<longlong2*>(p.slots + t0) = make_longlong2(slot[0], slot[1]);
-      *reinterpret_cast<longlong2*>(p.slots + t0 + 2) = make_longlong2(slot[2], slot[3]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (t0 + i < p.max_tokens) {
-          p.positions[t0 + i] = pos[i];
-          p.slots[t0 + i] = slot[i];
-        }
+        const unsigned to = static_cast<unsigned>(count) + push[at(s)] + j;
+        if (j < held && to < static_cast<unsigned>(nb)) ring(to) = row[j];
+        if (j < now) row[j] = ring(pop[at(s)] + j);
       }
     }
   }
 }
 
 cudaError_t launch_plan(const PlanParams& p, cudaStream_t stream) {
-  const int smem = 3 * (p.num_seqs + 1) * static_cast<int>(sizeof(int));
+  const int smem = 3 * padded(p.num_seqs + 1) * static_cast<int>(sizeof(int));
   const cudaError_t e = ensure_smem_optin(reinterpret_cast<const void*>(plan_kernel), smem);
   if (e != cudaSuccess) return e;
-  // 4 tokens a thread; 8 threads a request for the finished rows
-  const long long threads = std::max<long long>((p.max_tokens + 3LL) / 4, 8LL * p.num_seqs);
+  // a token a thread; 8 threads a request for the finished rows
+  const long long threads = std::max<long long>(p.max_tokens, 8LL * p.num_seqs);
   const long long blocks = (threads + kPlanThreads - 1) / kPlanThreads;
-  const int grid = static_cast<int>(std::min<long long>(std::max<long long>(blocks, 1), sm_count()));
-  plan_kernel<<<grid, kPlanThreads, smem, stream>>>(p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>(std::max<long long>(blocks, 1), sm_count())));
+  cfg.blockDim = dim3(kPlanThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  // placed while the kernel before finishes (it waits for it), and not triggering itself:
+  // the decode reads lengths and tables before its own wait
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, plan_kernel, p);
 }
 
 }  // namespace step
