@@ -119,6 +119,7 @@ __global__ void __launch_bounds__(256) page_bounds_kernel(const BoundsParams p) 
   constexpr int CPR = D / N;              // lanes (16-byte chunks) a row takes: 8, 16 or 32
   constexpr int RPI = 32 / CPR;           // rows a warp reads at once
   constexpr int IT = BS / RPI;            // reads a page takes
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31;
   const long long item = blockIdx.x * 8LL + (threadIdx.x >> 5);
   const int h = static_cast<int>(item % p.kv_heads);
@@ -195,12 +196,19 @@ __global__ void __launch_bounds__(256) page_bounds_kernel(const BoundsParams p) 
 template <typename T>
 static cudaError_t launch_bounds_t(const BoundsParams& p, int d, int bs, cudaStream_t st) {
   const long long items = (p.tokens + 31LL) / 32 * p.kv_heads;
-  const dim3 grid(static_cast<unsigned>((items + 7) / 8));
-#define FE_CASE(D_, BS_, L_)                                     \
-  if (d == D_ && bs == BS_ && p.kv_layout == L_) {               \
-    page_bounds_kernel<T, D_, BS_, L_><<<grid, 256, 0, st>>>(p); \
-    return cudaGetLastError();                                   \
-  }
+  // placed while the kernel before finishes, which it waits for before it reads anything
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((items + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+#define FE_CASE(D_, BS_, L_)                     \
+  if (d == D_ && bs == BS_ && p.kv_layout == L_) \
+    return cudaLaunchKernelEx(&cfg, page_bounds_kernel<T, D_, BS_, L_>, p);
   FE_CASE(64, 16, paged::kKvFlat)
   FE_CASE(64, 32, paged::kKvFlat)
   FE_CASE(128, 16, paged::kKvFlat)
