@@ -60,6 +60,7 @@ struct PagedArgs {
   int S, H, Hkv, d, bs, max_ctx, maxb, num_blocks;
   float scale;
   int kv_layout = fe::paged::kKvFlat;
+  int serial = 0;  // block_tables and context_lens come from the kernel before
   const float* rope_cos = nullptr;
   const float* rope_sin = nullptr;
   int rope_max_pos = 0;
@@ -192,6 +193,7 @@ int paged_tc_run(const PagedArgs& a, const DecodePlan& pl, float* ws, cudaStream
     p.rope_cos = a.rope_cos;
     p.rope_sin = a.rope_sin;
     p.rope_max_pos = a.rope_max_pos;
+    p.serial = a.serial;
     p.err = err;
     for (int r = 0; r < fe::paged::kMaxRanks; ++r) p.xbuf[r] = pl.xbuf[r];
     p.xworld = pl.xworld;
@@ -603,6 +605,7 @@ int fe_sparse_paged_attention(const void* q, const void* kc, const void* vc, voi
   if (static_cast<long long>(num_blocks) * Hkv * bs > INT_MAX) return kErr;
   a.num_blocks = num_blocks * Hkv;
   a.kv_layout = kv_layout;
+  a.serial = 1;
   const int rc = dtype == 0 ? paged_check<__nv_bfloat16>(a)
                  : dtype == 1 ? paged_check<half>(a)
                  : dtype == 2 ? paged_check<float>(a)

@@ -1541,7 +1541,7 @@ static cudaError_t launch_cfg(const Params& p, const void* kc, const void* vc, l
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = p.serial ? 0 : 1;
   return cudaLaunchKernelEx(&cfg, kern, km, vm, pp);
 }
 

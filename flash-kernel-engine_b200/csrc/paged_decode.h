@@ -72,6 +72,8 @@ struct Params {
   const float* rope_cos;
   const float* rope_sin;
   int rope_max_pos;
+  int serial;              // 1: not placed before the kernel before has finished (that kernel
+                           // writes block_tables and context_lens)
   unsigned* err;           // device error word
   long long dbg_kv_rows;   // rows of the K/V tensor maps (bounds checks in debug builds)
   // KV-range exchange (partials mode with xworld > 0): every finished partial row is

@@ -18,10 +18,11 @@
 // paged_decode.cu.
 //
 // Choice. A score is kept as an ordered 32-bit key, with the largest key of every 8 pages.
-// The m-th largest of those maxima is a lower bound of the m-th largest key, so that only
-// groups that reach it are looked at again (where there are at least 2 m groups): a few
-// hundred of thousands. The threshold then comes from histograms of their keys, refined
-// until the wanted count ends at a bin's edge or a bin is a single key.
+// Up to 8 pages a thread are held in registers, and the K-th largest key is found bit by bit
+// from the first bit in which the keys differ, one barrier a bit. Longer rows first look at
+// the groups' maxima in the same way: the m-th largest of them is a lower bound of the m-th
+// largest key, so that only groups that reach it matter: a few hundred of thousands. Where
+// those are too many (equal scores, say), all keys are read again for every bit.
 //
 // Two launches. page_score_kernel reads the boxes: one CTA an SM takes an equal share of all
 // sequences' 16-page tiles, whatever their lengths, and all KV heads of a tile at once, whose
@@ -52,8 +53,6 @@ namespace cg = cooperative_groups;
 namespace fe {
 namespace step {
 
-constexpr int kBinBits = 11;
-constexpr int kBins = 1 << kBinBits;
 constexpr unsigned kForced = 0xffffffffu;  // key of an always-chosen page, above every score
 constexpr float kInf = __builtin_huge_valf();
 constexpr int kMaxCtas = 8;            // of one (sequence, KV head)
@@ -63,8 +62,6 @@ constexpr int kScoreStages = 32;       // and tiles
 constexpr int kScoreSeqs = 4096;       // most sequences of one launch of it
 constexpr int kMaxFusedPages = 8192;   // most chosen pages whose list fits shared memory
 constexpr int kGroup = 8;              // pages whose largest key is kept
-constexpr int kMaxGroups = 8192;       // more groups of a row stay in global memory
-constexpr int kMaxKeys = 8192;         // keys looked at again that shared memory takes
 
 // Order-preserving map of a float (no NaN, no -0) to 32 bits.
 __device__ __forceinline__ unsigned key_of(float x) {
@@ -234,335 +231,250 @@ __device__ __forceinline__ void score_tile(const SelectParams& p, int pages,
 
 template <int NTHR>
 struct SelectShared {
-  unsigned hist[kBins];
   unsigned count[2][(NTHR / 32 + 3) / 4 * 4];
-  unsigned sums[NTHR / 32], above[NTHR / 32], equal[NTHR / 32];
-  unsigned lo, hi;             // ends of the keys in question
-  unsigned bin, over, in_bin;  // result of one histogram
+  unsigned above[NTHR / 32], equal[NTHR / 32];
+  int groups[NTHR];  // groups that matter
 };
 
-// The shared memory that a choice works in.
-struct Workspace {
-  unsigned* keys;    // [key_cap]
-  unsigned* maxima;  // [group_cap]
-  int* groups;       // [group_cap] groups looked at again
-  int key_cap, group_cap;
-};
-
-// Of the n keys key(i): the bin of [lo, hi] cut into kBins that holds the rem-th largest of
-// those inside. Leaves hist zeroed.
-template <int NTHR, typename Key>
-__device__ __forceinline__ void find_bin(SelectShared<NTHR>& sh, int n, Key key, unsigned lo,
-                                         unsigned hi, int shift, unsigned rem) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  constexpr int NW = NTHR / 32, BPT = kBins / NTHR;
-  for (int i = tid; i < n; i += NTHR) {
-    const unsigned k = key(i);
-    if (k >= lo && k <= hi) atomicAdd(&sh.hist[(k - lo) >> shift], 1u);
-  }
-  __syncthreads();
-  // this thread's bins, the highest ones first over the threads
-  unsigned c[BPT], sum = 0;
-  const int b0 = kBins - (tid + 1) * BPT;
-#pragma unroll
-  for (int i = 0; i < BPT; i += 4) {
-    uint4* h = reinterpret_cast<uint4*>(sh.hist + b0 + i);
-    const uint4 v = *h;
-    *h = make_uint4(0, 0, 0, 0);
-    c[i] = v.x;
-    c[i + 1] = v.y;
-    c[i + 2] = v.z;
-    c[i + 3] = v.w;
-    sum += v.x + v.y + v.z + v.w;
-  }
-  unsigned inc = sum;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const unsigned v = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += v;
-  }
-  if (lane == 31) sh.sums[warp] = inc;
-  __syncthreads();
-  unsigned over = inc - sum;
-#pragma unroll
-  for (int w = 0; w < NW; ++w) over += w < warp ? sh.sums[w] : 0;
-  if (over < rem && rem <= over + sum) {
-    bool done = false;
-#pragma unroll
-    for (int i = BPT - 1; i >= 0; --i) {
-      if (!done && rem <= over + c[i]) {
-        sh.bin = b0 + i;
-        sh.over = over;
-        sh.in_bin = c[i];
-        done = true;
-      }
-      over += c[i];
-    }
-  }
-  __syncthreads();
-}
-
-__device__ __forceinline__ int bin_shift(unsigned lo, unsigned hi) {
-  return lo == hi ? 0 : max(0, 32 - __clz(hi - lo) - kBinBits);
-}
-
-// put(place, page) for the K chosen pages of a row of at most NTHR * J pages, in ascending
-// order: warp w holds the keys of pages [32 J w, 32 J (w + 1)) in registers. The K-th
-// largest key is found bit by bit from the top, one barrier a bit; it ends early where a
-// prefix has exactly K keys at or above it.
-template <int NTHR, int J, typename Shared, typename Put>
-__device__ __forceinline__ void choose_in_registers(Shared& sh, const unsigned* gkeys, int pages,
-                                                    int K, Put put) {
-  constexpr int NW = NTHR / 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int first = warp * 32 * J + lane;
-  unsigned k[J];
-#pragma unroll
-  for (int j = 0; j < J; ++j) k[j] = first + j * 32 < pages ? __ldcg(gkeys + first + j * 32) : 0;
-  // the sum of a count over the block: counts of round i in row i & 1
-  auto total = [&](unsigned c, int i) {
-    c = __reduce_add_sync(0xffffffffu, c);
-    if constexpr (NW == 1) return c;
-    if (lane == 0) sh.count[i & 1][warp] = c;
+// The sum of a count over the block; row: alternates from call to call.
+template <int NW, typename Shared>
+__device__ __forceinline__ unsigned block_count(Shared& sh, unsigned c, int row) {
+  c = __reduce_add_sync(0xffffffffu, c);
+  if constexpr (NW > 1) {
+    if ((threadIdx.x & 31) == 0) sh.count[row & 1][threadIdx.x >> 5] = c;
     __syncthreads();
-    unsigned all = 0;
+    c = 0;
 #pragma unroll
-    for (int w = 0; w < NW; w += 4) {
-      const uint4 v = *reinterpret_cast<const uint4*>(&sh.count[i & 1][w]);
-      all += v.x + v.y + v.z + v.w;
+    for (int w = 0; w < NW; ++w) c += sh.count[row & 1][w];
+  }
+  return c;
+}
+
+// The smallest and the largest of a value of each thread over the block.
+template <int NW, typename Shared>
+__device__ __forceinline__ void block_range(Shared& sh, unsigned& lo, unsigned& hi) {
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if constexpr (NW > 1) {
+    __syncthreads();  // sh.above and sh.equal are read
+    if ((threadIdx.x & 31) == 0) {
+      sh.above[threadIdx.x >> 5] = lo;
+      sh.equal[threadIdx.x >> 5] = hi;
     }
-    return all;
-  };
-  unsigned thr = 0;  // chosen are the keys above thr and the first `need` equal to it
-  int need = -1;
-  for (int bit = 31; bit >= 0; --bit) {
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      lo = min(lo, sh.above[w]);
+      hi = max(hi, sh.equal[w]);
+    }
+  }
+}
+
+// A threshold with at least K and at most `most` keys at or above it where there is one, else
+// the K-th largest key. More than the always-chosen ones are wanted, so that it is one of
+// the others, which lie between lo and hi. count(at): this thread's keys at or above `at`.
+template <int NW, typename Shared, typename Count>
+__device__ __forceinline__ unsigned find_threshold(Shared& sh, unsigned lo, unsigned hi,
+                                                   unsigned K, unsigned most, Count count) {
+  const int bits = 32 - __clz(lo ^ hi);  // those below the first one in which the keys differ
+  unsigned thr = bits == 32 ? 0 : (hi >> bits) << bits;
+  for (int bit = bits - 1; bit >= 0; --bit) {
     const unsigned at = thr | (1u << bit);
-    unsigned c = 0;
-#pragma unroll
-    for (int j = 0; j < J; ++j) c += k[j] >= at;
-    c = total(c, bit);
-    if (c >= static_cast<unsigned>(K)) thr = at;
-    if (c == static_cast<unsigned>(K)) {
-      thr -= 1;
-      need = 0;
-      break;
+    const unsigned c = block_count<NW>(sh, count(at), bit);
+    if (c >= K) {
+      thr = at;
+      if (c <= most) break;
     }
   }
-  unsigned above = 0, equal = 0;
-#pragma unroll
-  for (int j = 0; j < J; ++j) {
-    above += k[j] > thr;
-    equal += k[j] == thr;
-  }
+  return thr;
+}
+
+// How many keys are above / equal to the threshold: in the warps before, and in all.
+struct Before {
+  unsigned above, equal, all_above, all_equal;
+};
+template <int NW, typename Shared>
+__device__ __forceinline__ Before block_before(Shared& sh, unsigned above, unsigned equal) {
   above = __reduce_add_sync(0xffffffffu, above);
   equal = __reduce_add_sync(0xffffffffu, equal);
-  unsigned a = 0, e = 0;  // in the warps before
+  Before b{0, 0, above, equal};
   if constexpr (NW > 1) {
-    if (lane == 0) {
+    const int warp = threadIdx.x >> 5;
+    __syncthreads();  // sh.above and sh.equal are read
+    if ((threadIdx.x & 31) == 0) {
       sh.above[warp] = above;
       sh.equal[warp] = equal;
     }
     __syncthreads();
-    unsigned all = 0;
+    b.all_above = b.all_equal = 0;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      a += w < warp ? sh.above[w] : 0;
-      e += w < warp ? sh.equal[w] : 0;
-      all += sh.above[w];
+      b.above += w < warp ? sh.above[w] : 0;
+      b.equal += w < warp ? sh.equal[w] : 0;
+      b.all_above += sh.above[w];
+      b.all_equal += sh.equal[w];
     }
-    above = all;
   }
-  if (need < 0) need = K - static_cast<int>(above);
-  const unsigned below = (1u << lane) - 1;
+  return b;
+}
+
+// 32 consecutive places of a warp: put(place in the list, i) where `k` is above thr, or equal
+// to it and among the first `need` equal ones. b moves on past them.
+template <typename Put>
+__device__ __forceinline__ void list_32(Before& b, unsigned k, unsigned thr, unsigned need, int i,
+                                        Put put) {
+  const unsigned below = (1u << (threadIdx.x & 31)) - 1;
+  const unsigned ma = __ballot_sync(0xffffffffu, k > thr);
+  const unsigned me = __ballot_sync(0xffffffffu, k == thr);
+  const unsigned e = b.equal + __popc(me & below);  // equal ones before this place
+  if (k > thr || (k == thr && e < need))
+    put(static_cast<int>(b.above + __popc(ma & below) + min(e, need)), i);
+  b.above += __popc(ma);
+  b.equal += __popc(me);
+}
+
+// Keys of up to NTHR * J places in registers: warp w holds places [32 J w, 32 J (w + 1)),
+// lane l those with place % 32 == l.
+template <int NTHR, int J>
+struct KeyRegisters {
+  static constexpr int NW = NTHR / 32;
+  unsigned k[J];
+  int first;
+  template <typename Key>
+  __device__ __forceinline__ void load(int n, Key key) {  // key(i): the key of place i < n
+    first = (threadIdx.x >> 5) * 32 * J + (threadIdx.x & 31);
+#pragma unroll
+    for (int j = 0; j < J; ++j) k[j] = first + j * 32 < n ? key(first + j * 32) : 0;
+  }
+  template <typename Shared>
+  __device__ __forceinline__ unsigned threshold(Shared& sh, unsigned K, unsigned most) const {
+    unsigned lo = kForced, hi = 0;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      if (k[j] != 0) lo = min(lo, k[j]);
+      if (k[j] != kForced) hi = max(hi, k[j]);
+    }
+    block_range<NW>(sh, lo, hi);
+    return find_threshold<NW>(sh, lo, hi, K, most, [&](unsigned at) {
+      unsigned c = 0;
+#pragma unroll
+      for (int j = 0; j < J; ++j) c += k[j] >= at;
+      return c;
+    });
+  }
+  template <typename Shared>
+  __device__ __forceinline__ Before before(Shared& sh, unsigned thr) const {
+    unsigned above = 0, equal = 0;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      above += k[j] > thr;
+      equal += k[j] == thr;
+    }
+    return block_before<NW>(sh, above, equal);
+  }
+  template <typename Put>
+  __device__ __forceinline__ void list(Before b, unsigned thr, unsigned need, Put put) const {
+#pragma unroll
+    for (int j = 0; j < J; ++j) list_32(b, k[j], thr, need, first + j * 32, put);
+  }
+};
+
+// put(place, i) for the K best of n places i in ascending order, `rem` of them not kForced.
+template <int NTHR, int J, typename Shared, typename Key, typename Put>
+__device__ __forceinline__ void choose_in_registers(Shared& sh, int n, unsigned K, unsigned rem,
+                                                    Key key, Put put) {
+  KeyRegisters<NTHR, J> r;
+  r.load(n, key);
+  const unsigned thr = rem > 0 ? r.threshold(sh, K, K) : kForced - 1;
+  const Before b = r.before(sh, thr);
+  r.list(b, thr, K - b.all_above, put);
+}
+
+// The groups of 8 pages that matter into sh.groups: those whose largest open key reaches a
+// lower bound of the rem-th largest open key, and those of always-chosen pages (outside
+// [first_end, last_beg)). Returns their number, which is above NTHR where they do not fit.
+template <int NTHR, int J>
+__device__ __forceinline__ int find_groups(SelectShared<NTHR>& sh, const unsigned* gmaxima, int ng,
+                                           unsigned rem, int first_end, int last_beg) {
+  KeyRegisters<NTHR, J> m;
+  m.load(ng, [&](int i) { return __ldcg(gmaxima + i); });
+  const unsigned thr = m.threshold(sh, rem, rem + rem / 4 + 8);
 #pragma unroll
   for (int j = 0; j < J; ++j) {
-    const unsigned ma = __ballot_sync(0xffffffffu, k[j] > thr);
-    const unsigned me = __ballot_sync(0xffffffffu, k[j] == thr);
-    const int ea = static_cast<int>(e) + __popc(me & below);  // equal ones before this page
-    if ((ma >> lane & 1) || ((me >> lane & 1) && ea < need))
-      put(static_cast<int>(a) + __popc(ma & below) + min(ea, need), first + j * 32);
-    a += __popc(ma);
-    e += __popc(me);
+    const int i = m.first + j * 32;
+    if (i < ng && (i < first_end || i >= last_beg)) m.k[j] = kForced;
   }
-}
-// The same for any row that fits, NTHR * 8 pages: by one warp up to 256 pages, where the
-// barriers would cost more than the longer turns.
-template <int NTHR, typename Put>
-__device__ __forceinline__ void choose_in_registers(SelectShared<NTHR>& sh, const unsigned* gkeys,
-                                                    int pages, int K, Put put) {
-  if (pages <= 256) {
-    if (threadIdx.x >= 32) return;
-    if (pages <= 128) choose_in_registers<32, 4>(sh, gkeys, pages, K, put);
-    else choose_in_registers<32, 8>(sh, gkeys, pages, K, put);
-  } else if (pages <= NTHR * 3) {
-    choose_in_registers<NTHR, 3>(sh, gkeys, pages, K, put);
-  } else {
-    choose_in_registers<NTHR, 8>(sh, gkeys, pages, K, put);
-  }
+  const Before b = m.before(sh, thr);
+  const int listed = static_cast<int>(b.all_above + b.all_equal);
+  if (listed <= NTHR) m.list(b, thr, b.all_equal, [&](int at, int i) { sh.groups[at] = i; });
+  __syncthreads();
+  return listed;
 }
 
-// put(place, page) for the K chosen pages of a row in ascending order (more than K pages).
-// gkeys, gmaxima: the row's keys and group maxima.
+// put(place, page) for the K chosen pages of a row (of more than K pages), in ascending order.
 template <int NTHR, typename Put>
 __device__ __forceinline__ void choose_pages(SelectShared<NTHR>& sh, const SelectParams& p,
-                                             const Seq& r, const Workspace& ws,
-                                             const unsigned* gkeys, const unsigned* gmaxima,
-                                             Put put) {
+                                             const Seq& r, const unsigned* gkeys,
+                                             const unsigned* gmaxima, Put put) {
   constexpr int NW = NTHR / 32;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int ng = (r.pages + kGroup - 1) / kGroup;
-  unsigned rem = p.num_pages - p.keep_first - p.keep_last;
-  const unsigned below = (1u << lane) - 1;
-  const unsigned* maxima = ws.maxima;
-  const bool fits = ng <= ws.group_cap;
-  if (!fits) maxima = gmaxima;
-
-  if (tid == 0) {
-    sh.lo = kForced;
-    sh.hi = 0;
+  const unsigned K = p.num_pages, rem = K - p.keep_first - p.keep_last;
+  const int n = r.pages, ng = (n + kGroup - 1) / kGroup;
+  auto key = [&](int i) { return __ldcg(gkeys + i); };
+  if (n <= 256) {  // one warp: the barriers would cost more than the longer turns
+    if (threadIdx.x >= 32) return;
+    if (n <= 128) choose_in_registers<32, 4>(sh, n, K, rem, key, put);
+    else choose_in_registers<32, 8>(sh, n, K, rem, key, put);
+    return;
   }
-  for (int i = tid; i < kBins; i += NTHR) sh.hist[i] = 0;
-  __syncthreads();
-  // ---- the groups to look at again: those whose largest key reaches `from`, and those of
-  // always-chosen pages
-  unsigned lo = kForced, hi = 0;
-  for (int i = tid; i < ng; i += NTHR) {
-    const unsigned k = __ldcg(gmaxima + i);
-    if (fits) ws.maxima[i] = k;
-    if (k) lo = min(lo, k);
-    hi = max(hi, k);
-  }
-  lo = __reduce_min_sync(0xffffffffu, lo);
-  hi = __reduce_max_sync(0xffffffffu, hi);
-  if (lane == 0) {
-    atomicMin(&sh.lo, lo);
-    atomicMax(&sh.hi, hi);
-  }
-  __syncthreads();
-  lo = sh.lo;
-  hi = sh.hi;
-  bool all = true;  // every group
-  unsigned from = 1;
+  if (n <= NTHR * 3) return choose_in_registers<NTHR, 3>(sh, n, K, rem, key, put);
+  if (n <= NTHR * 8) return choose_in_registers<NTHR, 8>(sh, n, K, rem, key, put);
   const int first_end = (p.keep_first + kGroup - 1) / kGroup;
-  const int last_beg = (r.pages - p.keep_last) / kGroup;
-  // groups [first_end, last_beg) have no always-chosen page
-  if (fits && 2 * static_cast<int>(rem) <= max(0, last_beg - first_end)) {
-    all = false;
-    if (rem > 0) {
-      const int shift = bin_shift(lo, hi);
-      find_bin<NTHR>(sh, ng, [&](int i) { return maxima[i]; }, lo, hi, shift, rem);
-      from = lo + (sh.bin << shift);
-    } else {
-      from = kForced;
+  const int last_beg = (n - p.keep_last) / kGroup;
+  if (rem > 0 && ng <= NTHR * 16 && static_cast<int>(rem) <= (last_beg - first_end) / 2) {
+    const int listed = ng <= NTHR * 3 ? find_groups<NTHR, 3>(sh, gmaxima, ng, rem, first_end, last_beg)
+                       : ng <= NTHR * 8
+                           ? find_groups<NTHR, 8>(sh, gmaxima, ng, rem, first_end, last_beg)
+                           : find_groups<NTHR, 16>(sh, gmaxima, ng, rem, first_end, last_beg);
+    if (listed <= NTHR) {
+      auto page = [&](int i) { return sh.groups[i / kGroup] * kGroup + i % kGroup; };
+      return choose_in_registers<NTHR, 8>(
+          sh, listed * kGroup, K, rem, [&](int i) { return key(page(i)); },
+          [&](int at, int i) { put(at, page(i)); });
     }
   }
-  int nv = ng;
-  if (!all) {
-    // their list, each warp over a range of the groups
-    auto wanted = [&](int i) {
-      return maxima[i] >= from || i < first_end || i >= last_beg;
-    };
-    const int span = ((ng + NW - 1) / NW + 31) / 32 * 32;
-    const int wb = min(ng, warp * span), we = min(ng, wb + span);
-    unsigned cnt = 0;
-    for (int i = wb + lane; i < we; i += 32) cnt += wanted(i);
-    cnt = __reduce_add_sync(0xffffffffu, cnt);
-    if (lane == 0) sh.above[warp] = cnt;
-    __syncthreads();
-    unsigned at = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      at += w < warp ? sh.above[w] : 0;
-      total += sh.above[w];
-    }
-    nv = total;
-    for (int i0 = wb; i0 < we; i0 += 32) {
-      const bool ok = i0 + lane < we && wanted(i0 + lane);
-      const unsigned m = __ballot_sync(0xffffffffu, ok);
-      if (ok) ws.groups[at + __popc(m & below)] = i0 + lane;
-      at += __popc(m);
-    }
-    __syncthreads();
-  }
-  // ---- their keys: place i of the list is page page_at(i)
-  const int n = nv * kGroup;
-  auto page_at = [&](int i) { return all ? i : ws.groups[i / kGroup] * kGroup + i % kGroup; };
-  const bool copied = n <= ws.key_cap;
-  if (copied) {
-    for (int i = tid; i < n; i += NTHR) ws.keys[i] = __ldcg(gkeys + page_at(i));
-    __syncthreads();
-  }
-  auto key = [&](int i) {
-    return copied ? ws.keys[i] : __ldcg(gkeys + page_at(i));
-  };
-  // ---- the threshold: chosen are the keys above thr and the first `need` equal to it
-  unsigned thr = kForced - 1, need = 0;
+  // all keys, read again for every bit
+  unsigned thr = kForced - 1;
   if (rem > 0) {
-    if (all) {
-      unsigned k0 = kForced;
-      for (int i = tid; i < n; i += NTHR) {
-        const unsigned k = key(i);
-        if (k) k0 = min(k0, k);
-      }
-      k0 = __reduce_min_sync(0xffffffffu, k0);
-      if (lane == 0) atomicMin(&sh.lo, k0);
-      __syncthreads();
-      lo = sh.lo;
-    } else {
-      lo = from;
+    unsigned lo = kForced, hi = 0;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < n; i += NTHR) {
+      const unsigned k = key(i);
+      lo = min(lo, k);
+      if (k != kForced) hi = max(hi, k);
     }
-    for (;;) {
-      if (lo == hi) {
-        thr = lo;
-        need = rem;
-        break;
-      }
-      const int shift = bin_shift(lo, hi);
-      find_bin<NTHR>(sh, n, key, lo, hi, shift, rem);
-      lo += sh.bin << shift;
-      rem -= sh.over;
-      if (sh.in_bin == rem) {  // the whole bin is chosen
-        thr = lo - 1;
-        break;
-      }
-      hi = min(hi, lo + ((1u << shift) - 1));
-    }
+    block_range<NW>(sh, lo, hi);
+    thr = find_threshold<NW>(sh, lo, hi, K, K, [&](unsigned at) {
+      unsigned c = 0;
+#pragma unroll 8
+      for (int i = threadIdx.x; i < n; i += NTHR) c += key(i) >= at;
+      return c;
+    });
   }
-  // ---- the list, each warp over a range of the keys
+  // each warp lists a range of them
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int span = ((n + NW - 1) / NW + 31) / 32 * 32;
-  const int wb = min(n, warp * span), we = min(n, wb + span);
-  unsigned na = 0, ne = 0;
-  for (int i = wb + lane; i < we; i += 32) {
+  const int beg = min(n, warp * span), end = min(n, beg + span);
+  unsigned above = 0, equal = 0;
+#pragma unroll 8
+  for (int i = beg + lane; i < end; i += 32) {
     const unsigned k = key(i);
-    na += k > thr;
-    ne += k == thr;
+    above += k > thr;
+    equal += k == thr;
   }
-  na = __reduce_add_sync(0xffffffffu, na);
-  ne = __reduce_add_sync(0xffffffffu, ne);
-  __syncthreads();  // sh.above is read
-  if (lane == 0) {
-    sh.above[warp] = na;
-    sh.equal[warp] = ne;
-  }
-  __syncthreads();
-  unsigned a = 0, e = 0;
-#pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    a += w < warp ? sh.above[w] : 0;
-    e += w < warp ? sh.equal[w] : 0;
-  }
-  if (na == 0 && (ne == 0 || e >= need)) return;  // uniform in the warp
-  for (int i0 = wb; i0 < we; i0 += 32) {
-    const int i = i0 + lane;
-    const unsigned k = i < we ? key(i) : 0;
-    const unsigned ma = __ballot_sync(0xffffffffu, i < we && k > thr);
-    const unsigned me = __ballot_sync(0xffffffffu, i < we && k == thr);
-    const unsigned ea = e + __popc(me & below);  // equal ones before this page
-    if ((ma >> lane & 1) || ((me >> lane & 1) && ea < need))
-      put(static_cast<int>(a + __popc(ma & below) + min(ea, need)), page_at(i));
-    a += __popc(ma);
-    e += __popc(me);
-  }
+  Before b = block_before<NW>(sh, above, equal);
+  const unsigned need = K - b.all_above;
+  for (int i = beg; i < end; i += 32)
+    list_32(b, i + lane < end ? key(i + lane) : 0, thr, need, i + lane, put);
 }
 
 // ---------------------------------------------------------------------------
@@ -944,16 +856,15 @@ __device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 
-// Bytes of the region that holds first the keys, then the warps' partial results.
+// Bytes of the warps' partial results.
 template <int D, int NT, int NTHR>
 constexpr int merge_bytes() {
   return NTHR / 32 * 8 * NT * (D + 4 + 2) * 4;
 }
 
-// Byte offsets of the fused kernel's shared memory; the first region holds the keys, group
-// maxima and lists of the choice, and then the warps' partial results.
+// Byte offsets of the fused kernel's shared memory after the warps' partial results.
 struct SparseSmem {
-  int key_cap, group_cap, chosen, got, total;
+  int chosen, got, total;
 };
 
 // Selection and attention of one (sequence, KV head) by a cluster of `ctas` CTAs.
@@ -961,13 +872,7 @@ template <typename T, int D, int NT, int NTHR>
 __global__ void __launch_bounds__(NTHR, NT == 2 ? 1 : 512 / NTHR) sparse_decode_kernel(const SelectParams p, int ctas, const SparseSmem lay) {
   constexpr int NW = NTHR / 32, HP = 8 * NT;
   extern __shared__ __align__(16) unsigned char dyn[];
-  __shared__ __align__(16) SelectShared<NTHR> sh;
-  Workspace ws;
-  ws.keys = reinterpret_cast<unsigned*>(dyn);
-  ws.maxima = ws.keys + lay.key_cap;
-  ws.groups = reinterpret_cast<int*>(ws.maxima + lay.group_cap);
-  ws.key_cap = lay.key_cap;
-  ws.group_cap = lay.group_cap;
+  __shared__ SelectShared<NTHR> sh;
   int* chosen = reinterpret_cast<int*>(dyn + lay.chosen);  // [num_pages]
   float* got_m = reinterpret_cast<float*>(dyn + lay.got);  // [ctas][HP] of every CTA
   float* got_l = got_m + ctas * HP;
@@ -983,18 +888,17 @@ __global__ void __launch_bounds__(NTHR, NT == 2 ? 1 : 512 / NTHR) sparse_decode_
   const int P = r.pages, n = min(P, K);
   int* sel = p.selected + static_cast<long long>(row) * K;
 
+  WarpAttention<T, D, NT> w;
+  w.init(static_cast<const T*>(p.q) + (static_cast<long long>(seq) * p.heads + kvh * G) * D, G);
+
   // ---- the chosen pages, in every CTA's shared memory
   if (P > K) {
     auto put = [&](int at, int page) {
       chosen[at] = page;
       if (rank == 0) sel[at] = page;
     };
-    const unsigned* keys = p.keys + row * p.key_stride;
-    if (P <= NTHR * 8) {
-      choose_in_registers<NTHR>(sh, keys, P, K, put);
-    } else {
-      choose_pages<NTHR>(sh, p, r, ws, keys, p.maxima + row * (p.key_stride / kGroup), put);
-    }
+    choose_pages<NTHR>(sh, p, r, p.keys + row * p.key_stride,
+                       p.maxima + row * (p.key_stride / kGroup), put);
   } else {
     for (int i = tid; i < K; i += NTHR) {
       if (i < P) chosen[i] = i;
@@ -1023,8 +927,6 @@ __global__ void __launch_bounds__(NTHR, NT == 2 ? 1 : 512 / NTHR) sparse_decode_
     }
     at = ((static_cast<long long>(b) * p.kv_heads + kvh) * p.block_size + half_ * 16) * D;
   };
-  WarpAttention<T, D, NT> w;
-  w.init(static_cast<const T*>(p.q) + (static_cast<long long>(seq) * p.heads + kvh * G) * D, G);
   {
     long long at = 0, at_next = 0;
     int limit = 0, limit_next = 0;
@@ -1053,7 +955,6 @@ __global__ void __launch_bounds__(NTHR, NT == 2 ? 1 : 512 / NTHR) sparse_decode_
   }
 
   // ---- joined over the warps, then over the cluster
-  __syncthreads();  // the keys are read: their region takes the partial results
   float* om = reinterpret_cast<float*>(dyn);  // [NW][HP]
   float* ol = om + NW * HP;                   // [NW][HP]
   float* oo = ol + NW * HP;                   // [NW][HP][D + 4]
@@ -1104,9 +1005,8 @@ __global__ void __launch_bounds__(NTHR, NT == 2 ? 1 : 512 / NTHR) sparse_decode_
 // Selection alone, a CTA a row: the block table (block * Hkv + head) and the length that
 // paged_decode.cu runs over.
 template <int NTHR>
-__global__ void __launch_bounds__(NTHR) page_select_kernel(const SelectParams p,
-                                                           const SparseSmem lay) {
-  extern __shared__ __align__(16) unsigned char dyn[];
+__global__ void __launch_bounds__(NTHR) page_select_kernel(const SelectParams p) {
+  __shared__ SelectShared<NTHR> sh;
   const int tid = threadIdx.x, row = blockIdx.x, K = p.num_pages;
   const int seq = row / p.kv_heads, kvh = row - seq * p.kv_heads;
   griddep_wait();
@@ -1130,19 +1030,8 @@ __global__ void __launch_bounds__(NTHR) page_select_kernel(const SelectParams p,
     return;
   }
   auto put = [&](int at, int page) { sel[at] = page; };
-  const unsigned* keys = p.keys + row * p.key_stride;
-  __shared__ __align__(16) SelectShared<NTHR> sh;
-  if (P <= NTHR * 8) {
-    choose_in_registers<NTHR>(sh, keys, P, K, put);
-  } else {
-    Workspace ws;
-    ws.keys = reinterpret_cast<unsigned*>(dyn);
-    ws.maxima = ws.keys + lay.key_cap;
-    ws.groups = reinterpret_cast<int*>(ws.maxima + lay.group_cap);
-    ws.key_cap = lay.key_cap;
-    ws.group_cap = lay.group_cap;
-    choose_pages<NTHR>(sh, p, r, ws, keys, p.maxima + row * (p.key_stride / kGroup), put);
-  }
+  choose_pages<NTHR>(sh, p, r, p.keys + row * p.key_stride,
+                     p.maxima + row * (p.key_stride / kGroup), put);
   __syncthreads();  // the list is written, and read back by its CTA
 #pragma unroll 4
   for (int i = tid; i < K; i += NTHR) blocks[i] = block(sel[i]);
@@ -1218,24 +1107,14 @@ static cudaError_t launch_scores(const SelectParams& all, cudaStream_t st) {
   return cudaSuccess;
 }
 
-// Shared memory of the choice (and of `partials` bytes in its place afterwards), of the
-// list of chosen pages, and of `got` bytes from the other CTAs.
-static SparseSmem smem_layout(const SelectParams& p, int partials, int list, int got) {
-  SparseSmem l;
-  l.key_cap = static_cast<int>(std::min<long long>(p.key_stride, kMaxKeys));
-  l.group_cap = static_cast<int>(std::min<long long>(p.key_stride / kGroup, kMaxGroups) + 3) / 4 * 4;
-  l.chosen = (std::max((l.key_cap + 2 * l.group_cap) * 4, partials) + 15) / 16 * 16;
-  l.got = l.chosen + (list + 3) / 4 * 16;
-  l.total = l.got + got;
-  return l;
-}
-
 template <typename T, int D, int NT, int NTHR>
 static cudaError_t launch_fused(const SelectParams& p, int ctas, cudaStream_t st) {
   auto kern = sparse_decode_kernel<T, D, NT, NTHR>;
   const int share = (p.heads / p.kv_heads * D + ctas - 1) / ctas;
-  const SparseSmem lay = smem_layout(p, merge_bytes<D, NT, NTHR>(), p.num_pages,
-                                     ctas > 1 ? ctas * (share + 16 * NT) * 4 : 0);
+  SparseSmem lay;
+  lay.chosen = (merge_bytes<D, NT, NTHR>() + 15) / 16 * 16;
+  lay.got = lay.chosen + (p.num_pages + 3) / 4 * 16;
+  lay.total = lay.got + (ctas > 1 ? ctas * (share + 16 * NT) * 4 : 0);
   const cudaError_t e = ensure_smem_optin(reinterpret_cast<const void*>(kern), lay.total);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg;
@@ -1245,16 +1124,12 @@ static cudaError_t launch_fused(const SelectParams& p, int ctas, cudaStream_t st
   return cudaLaunchKernelEx(&cfg, kern, p, ctas, lay);
 }
 
-template <int NTHR>
 static cudaError_t launch_select(const SelectParams& p, cudaStream_t st) {
-  auto kern = page_select_kernel<NTHR>;
-  const SparseSmem lay = smem_layout(p, 0, 0, 0);
-  const cudaError_t e = ensure_smem_optin(reinterpret_cast<const void*>(kern), lay.total);
-  if (e != cudaSuccess) return e;
+  constexpr int NTHR = 512;
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr[2];
-  launch_config(cfg, attr, static_cast<long long>(p.num_seqs) * p.kv_heads, NTHR, lay.total, 1, st);
-  return cudaLaunchKernelEx(&cfg, kern, p, lay);
+  launch_config(cfg, attr, static_cast<long long>(p.num_seqs) * p.kv_heads, NTHR, 0, 1, st);
+  return cudaLaunchKernelEx(&cfg, page_select_kernel<NTHR>, p);
 }
 
 template <typename T, int D>
@@ -1278,7 +1153,7 @@ static cudaError_t launch_d(SelectParams& p, bool fused, cudaStream_t st) {
       return launch_fused<T, D, 1, 512>(p, ctas, st);
     }
   }
-  return launch_select<512>(p, st);
+  return launch_select(p, st);
 }
 
 template <typename T>

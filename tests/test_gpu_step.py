@@ -445,6 +445,15 @@ def test_sparse_ties_go_to_the_lower_page(ctx):
     check_sparse(few, 21)
 
 
+def test_sparse_ties_in_a_long_row():
+    """More equal scores than the registers of a CTA hold."""
+    p = make_sparse(14, [150001], 2, 1, 64, 16, BF16)
+    check_sparse(dict(p, q=np.zeros_like(p["q"])), 9)
+    few = dict(p, k=p["k"][np.arange(len(p["k"])) % 3])
+    check_sparse(few, 33)
+    check_sparse(p, 33, 20, 12)
+
+
 def test_sparse_scores_below_zero():
     """Keys that point away from the query: all scores negative, the nearest to zero win."""
     p = make_sparse(4, [700, 650], 2, 1, 64, 16, F32)
