@@ -231,36 +231,36 @@ __device__ __forceinline__ void score_tile(const SelectParams& p, int pages,
 
 template <int NTHR>
 struct SelectShared {
-  unsigned count[2][(NTHR / 32 + 3) / 4 * 4];
+  unsigned count[32];
   unsigned above[NTHR / 32], equal[NTHR / 32];
   int groups[NTHR];  // groups that matter
 };
 
-// The sum of a count over the block; row: alternates from call to call.
+// The sum of a count over the block in turn `row`, each of which is used once after
+// block_range.
 template <int NW, typename Shared>
 __device__ __forceinline__ unsigned block_count(Shared& sh, unsigned c, int row) {
   c = __reduce_add_sync(0xffffffffu, c);
   if constexpr (NW > 1) {
-    if ((threadIdx.x & 31) == 0) sh.count[row & 1][threadIdx.x >> 5] = c;
+    if ((threadIdx.x & 31) == 0) atomicAdd(&sh.count[row], c);
     __syncthreads();
-    c = 0;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) c += sh.count[row & 1][w];
+    c = sh.count[row];
   }
   return c;
 }
 
-// The smallest and the largest of a value of each thread over the block.
+// The smallest and the largest of a value of each thread over the block. Clears the counts.
 template <int NW, typename Shared>
 __device__ __forceinline__ void block_range(Shared& sh, unsigned& lo, unsigned& hi) {
   lo = __reduce_min_sync(0xffffffffu, lo);
   hi = __reduce_max_sync(0xffffffffu, hi);
   if constexpr (NW > 1) {
-    __syncthreads();  // sh.above and sh.equal are read
+    __syncthreads();  // sh.above, sh.equal and sh.count are read
     if ((threadIdx.x & 31) == 0) {
       sh.above[threadIdx.x >> 5] = lo;
       sh.equal[threadIdx.x >> 5] = hi;
     }
+    if (threadIdx.x < 32) sh.count[threadIdx.x] = 0;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
