@@ -243,6 +243,22 @@ def test_append_many_tokens_spread_over_the_gpu():
     check_append(6, 2500, 5, 1, 64, BF16, rotary=64)
 
 
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
+@pytest.mark.parametrize("kw", [
+    dict(H=6, Hkv=2, d=128, rotary=128, holes=True), dict(H=5, Hkv=3, d=64, rotary=64, pad=16),
+    dict(H=6, Hkv=2, d=128, rotary=None, interleaved=False),
+    dict(H=4, Hkv=4, d=256, rotary=256, weights=None, interleaved=False),
+    dict(H=2, Hkv=1, d=128, rotary=128, weights="fp32", bs=7),
+    dict(H=6, Hkv=2, d=128, rotary=64, interleaved=False), dict(H=40, Hkv=8, d=256, rotary=256),
+    dict(H=3, Hkv=1, d=128, rotary=128, layout="vllm")])
+def test_append_many_tokens(dt, kw):
+    """More than four tokens an SM: the ring of token rows, and what it does not take."""
+    if dt == F32 and "layout" in kw:
+        pytest.skip("the fp32 cache takes the flat layout")
+    check_append(7, 643, dt=dt, **kw)
+    assert fe().device_errors() == 0
+
+
 def test_append_norm_of_zero_and_of_large_rows():
     """An all-zero head stays zero, and a row whose squares pass bf16 stays finite."""
     d, bs = 128, 16
@@ -427,6 +443,11 @@ def test_sparse_many_rows(H, Hkv, d, bs):
     check_sparse(make_sparse(12, g.integers(0, 700, 45), H, Hkv, d, bs, BF16), 5)
 
 
+def test_sparse_more_sequences_than_a_score_launch_takes():
+    g = np.random.default_rng(15)
+    check_sparse(make_sparse(15, g.integers(0, 80, 4099), 2, 1, 64, 16, BF16), 2)
+
+
 def test_sparse_many_pages_chosen():
     """A list longer than the attention's shared memory holds goes through the paged decode."""
     check_sparse(make_sparse(13, [140000, 90], 2, 1, 64, 16, BF16), 8300)
@@ -602,3 +623,24 @@ def test_step_in_a_cuda_graph():
     for k in before:
         assert torch.equal(eager[k], graphed[k]), k
     assert F.device_errors() == 0
+
+
+def test_serving_example_runs():
+    """The example's loop, small: with as many pages as the longest request has, the sparse
+    decode is the dense one; with fewer it attends to fewer and stays near."""
+    import os
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    sys.path.insert(0, os.path.join(root, "examples"))
+    try:
+        import serving_step
+    finally:
+        sys.path.pop(0)
+    kw = dict(steps=14, requests=6, heads=8, kv_heads=2, d=64, max_len=512, prompt=(20, 200),
+              tokens_per_step=256, quiet=True)
+    whole = serving_step.serve(pages=32, **kw)
+    few = serving_step.serve(pages=3, **kw)
+    assert whole["errors"] == 0 and few["errors"] == 0 and whole["finite"] and few["finite"]
+    assert whole["tokens"] == few["tokens"] > 14 * 3
+    assert whole["share"] == 1 and whole["diff"] < 2 ** -7
+    assert few["share"] < 0.9 and few["diff"] < 1
