@@ -55,7 +55,8 @@ namespace step {
 
 constexpr unsigned kForced = 0xffffffffu;  // key of an always-chosen page, above every score
 constexpr float kInf = __builtin_huge_valf();
-constexpr int kMaxCtas = 8;            // of one (sequence, KV head)
+constexpr int kMaxCtas = 8;            // of one (sequence, KV head): the portable cluster; of
+                                       // clusters of 16 only four were resident at a time
 constexpr int kScoreWarps = 16;        // of a CTA of the score launch
 constexpr int kScoreRing = 150 * 1024; // bytes of boxes of a CTA in flight, at most
 constexpr int kScoreStages = 32;       // and tiles
@@ -485,6 +486,10 @@ __device__ __forceinline__ void choose_pages(SelectShared<NTHR>& sh, const Selec
 // a ring of tiles; consumer warp w scores head w % head_group of every (16 / head_group)th
 // tile. A tile's place in the ring always belongs to the same consumer warps (`stages` is a
 // multiple of 16 / head_group), so a parity wait cannot be satisfied by an older phase.
+// HBM bound once it streams: four contexts of 131072 tokens (67 MB of boxes) take 15 us, of
+// which 1.6 go to the prefix sum and 3 to the block table, the query and the first tiles;
+// then a CTA takes 46 GB/s, 6.8 TB/s in all. With the boxes read into registers, one row a
+// CTA, it took 20 us: 256-byte reads of one head at a time, and two tiles a warp in flight.
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * (kScoreWarps + 1), 1)
     page_score_kernel(const SelectParams p, int head_group, int stages) {
@@ -867,7 +872,10 @@ struct SparseSmem {
   int chosen, got, total;
 };
 
-// Selection and attention of one (sequence, KV head) by a cluster of `ctas` CTAs.
+// Selection and attention of one (sequence, KV head) by a cluster of `ctas` CTAs. Of 26 us for
+// four contexts of 131072 tokens and 256 pages (67 MB of keys and values), the choice takes
+// 7.5, the attention 13 (5 TB/s on 128 SMs) and the joins 2.7; 512 rows of 64 pages (268 MB)
+// take 47 us in the attention, 5.7 TB/s.
 template <typename T, int D, int NT, int NTHR>
 __global__ void __launch_bounds__(NTHR, NT == 2 ? 1 : 512 / NTHR) sparse_decode_kernel(const SelectParams p, int ctas, const SparseSmem lay) {
   constexpr int NW = NTHR / 32, HP = 8 * NT;

@@ -1,7 +1,8 @@
 // Umbrella header of the B200 inference-attention library -- drop-in for the
 // hot-path part of the reference's include/flash_engine.h:1-31: the attention
-// headers, the rotary embedding that feeds attention (fused_rope.cuh) and the CUDA
-// graph runner used to capture decode steps. The reference's other kernels (RMSNorm,
+// headers, the rotary embedding that feeds attention (fused_rope.cuh), the serving-step
+// operators around the paged decode (serving_step.cuh) and the CUDA graph runner used to
+// capture decode steps. The reference's other kernels (RMSNorm,
 // activations, speculative decoding, quantized GEMM, cross-entropy) and its memory pool
 // are not part of this library.
 #pragma once
@@ -13,6 +14,7 @@
 #include "paged_attention.cuh"
 #include "flash_engine_c.h"
 #include "fused_rope.cuh"
+#include "serving_step.cuh"
 
 namespace flash_engine {
 

@@ -551,6 +551,36 @@ def test_sparse_flags_a_block_out_of_range():
         assert fe().device_errors() == _lib.ERR_BAD_BLOCK
 
 
+def test_offsets_past_32_bits():
+    """The operators at the end of a cache of more than 2^32 bytes and 2^31 elements give what
+    they give in a small one."""
+    H, Hkv, d, bs, T = 8, 4, 128, 16, 75
+    small, nb = 5, 262144 + 500
+    g = torch.Generator(device="cuda").manual_seed(3)
+    qkv = torch.randn((T, (H + 2 * Hkv) * d), device="cuda", generator=g).to(BF16)
+    pos = torch.arange(T, dtype=torch.int32, device="cuda")
+    order = torch.tensor([3, 0, 4, 2, 1], device="cuda")
+    q = qkv[:, :H * d].view(T, H, d)[-1:].contiguous()
+    lens = torch.tensor([T], dtype=torch.int32, device="cuda")
+    got = []
+    for blocks in (small, nb):
+        # the big cache is not cleared: only the blocks in use are looked at
+        kc, vc = (torch.empty((blocks, Hkv, bs, d), dtype=BF16, device="cuda") for _ in range(2))
+        table = order + blocks - small
+        kc[-small:], vc[-small:] = 0, 0
+        pb = fe().new_page_bounds(blocks, Hkv, d, "cuda")
+        slots = table[pos.long() // bs] * bs + pos.long() % bs
+        qa = fe().paged_qkv_append(qkv, kc, vc, pos, slots, H, bs, page_bounds=pb)
+        out, sel = fe().sparse_paged_attention(q, kc, vc, pb, table.int().view(1, -1), lens, 3, bs)
+        got.append([x.clone() for x in (qa, kc[-small:], vc[-small:], pb.values[-small:],
+                                        pb.scales[-small:], out, sel)])
+        del kc, vc
+    assert nb * Hkv * bs * d > 2 ** 31
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert fe().device_errors() == 0
+
+
 def test_sparse_on_another_stream_and_repeated():
     p = make_sparse(10, [3000, 100], 8, 2, 64, 16, BF16)
     a = check_sparse(p, 9, stream=torch.cuda.Stream())
