@@ -21,8 +21,8 @@
 // Up to 8 pages a thread are held in registers, and the K-th largest key is found bit by bit
 // from the first bit in which the keys differ, one barrier a bit. Longer rows first look at
 // the groups' maxima in the same way: the m-th largest of them is a lower bound of the m-th
-// largest key, so that only groups that reach it matter: a few hundred of thousands. Where
-// those are too many (equal scores, say), all keys are read again for every bit.
+// largest key, so that only keys that reach it matter: a few hundred of thousands, one a
+// thread. Where those are too many (equal scores, say), all keys are read again for every bit.
 //
 // Two launches. page_score_kernel reads the boxes: one CTA an SM takes an equal share of all
 // sequences' 16-page tiles, whatever their lengths, and all KV heads of a tile at once, whose
@@ -234,7 +234,9 @@ template <int NTHR>
 struct SelectShared {
   unsigned count[32];
   unsigned above[NTHR / 32], equal[NTHR / 32];
-  int groups[NTHR];  // groups that matter
+  int groups[NTHR];    // groups that matter
+  unsigned key[NTHR];  // candidates, and the pages they are of
+  int page[NTHR];
 };
 
 // The sum of a count over the block in turn `row`, each of which is used once after
@@ -319,8 +321,8 @@ __device__ __forceinline__ Before block_before(Shared& sh, unsigned above, unsig
   return b;
 }
 
-// 32 consecutive places of a warp: put(place in the list, i) where `k` is above thr, or equal
-// to it and among the first `need` equal ones. b moves on past them.
+// 32 consecutive places of a warp: put(place in the list, i, k) where `k` is above thr, or
+// equal to it and among the first `need` equal ones. b moves on past them.
 template <typename Put>
 __device__ __forceinline__ void list_32(Before& b, unsigned k, unsigned thr, unsigned need, int i,
                                         Put put) {
@@ -329,7 +331,7 @@ __device__ __forceinline__ void list_32(Before& b, unsigned k, unsigned thr, uns
   const unsigned me = __ballot_sync(0xffffffffu, k == thr);
   const unsigned e = b.equal + __popc(me & below);  // equal ones before this place
   if (k > thr || (k == thr && e < need))
-    put(static_cast<int>(b.above + __popc(ma & below) + min(e, need)), i);
+    put(static_cast<int>(b.above + __popc(ma & below) + min(e, need)), i, k);
   b.above += __popc(ma);
   b.equal += __popc(me);
 }
@@ -388,18 +390,47 @@ __device__ __forceinline__ void choose_in_registers(Shared& sh, int n, unsigned 
   r.load(n, key);
   const unsigned thr = rem > 0 ? r.threshold(sh, K, K) : kForced - 1;
   const Before b = r.before(sh, thr);
-  r.list(b, thr, K - b.all_above, put);
+  r.list(b, thr, K - b.all_above, [&](int at, int i, unsigned) { put(at, i); });
+}
+
+// put(place, page) for the K best of n <= NTHR candidates in sh.key, one a thread, `rem` of
+// them not kForced: the barrier itself counts.
+template <int NTHR, typename Put>
+__device__ __forceinline__ void choose_candidates(SelectShared<NTHR>& sh, int n, unsigned K,
+                                                  unsigned rem, Put put) {
+  constexpr int NW = NTHR / 32;
+  const int tid = threadIdx.x;
+  const unsigned k = tid < n ? sh.key[tid] : 0;
+  unsigned thr = kForced - 1;
+  if (rem > 0) {
+    unsigned lo = k != 0 ? k : kForced, hi = k != kForced ? k : 0;
+    block_range<NW>(sh, lo, hi);
+    const int bits = 32 - __clz(lo ^ hi);
+    thr = bits == 32 ? 0 : (hi >> bits) << bits;
+    for (int bit = bits - 1; bit >= 0; --bit) {
+      const unsigned at = thr | (1u << bit);
+      const unsigned c = __syncthreads_count(k >= at);
+      if (c >= K) {
+        thr = at;
+        if (c == K) break;
+      }
+    }
+  }
+  Before b = block_before<NW>(sh, k > thr, k == thr);
+  list_32(b, k, thr, K - b.all_above, tid,
+          [&](int at, int i, unsigned) { put(at, sh.page[i]); });
 }
 
 // The groups of 8 pages that matter into sh.groups: those whose largest open key reaches a
-// lower bound of the rem-th largest open key, and those of always-chosen pages (outside
-// [first_end, last_beg)). Returns their number, which is above NTHR where they do not fit.
+// lower bound of the rem-th largest open key (thr), and those of always-chosen pages
+// (outside [first_end, last_beg)). Returns their number, above NTHR where they do not fit.
 template <int NTHR, int J>
 __device__ __forceinline__ int find_groups(SelectShared<NTHR>& sh, const unsigned* gmaxima, int ng,
-                                           unsigned rem, int first_end, int last_beg) {
+                                           unsigned rem, int first_end, int last_beg,
+                                           unsigned& thr) {
   KeyRegisters<NTHR, J> m;
   m.load(ng, [&](int i) { return __ldcg(gmaxima + i); });
-  const unsigned thr = m.threshold(sh, rem, rem + rem / 4 + 8);
+  thr = m.threshold(sh, rem, rem + rem / 4 + 8);
 #pragma unroll
   for (int j = 0; j < J; ++j) {
     const int i = m.first + j * 32;
@@ -407,7 +438,7 @@ __device__ __forceinline__ int find_groups(SelectShared<NTHR>& sh, const unsigne
   }
   const Before b = m.before(sh, thr);
   const int listed = static_cast<int>(b.all_above + b.all_equal);
-  if (listed <= NTHR) m.list(b, thr, b.all_equal, [&](int at, int i) { sh.groups[at] = i; });
+  if (listed <= NTHR) m.list(b, thr, b.all_equal, [&](int at, int i, unsigned) { sh.groups[at] = i; });
   __syncthreads();
   return listed;
 }
@@ -432,15 +463,26 @@ __device__ __forceinline__ void choose_pages(SelectShared<NTHR>& sh, const Selec
   const int first_end = (p.keep_first + kGroup - 1) / kGroup;
   const int last_beg = (n - p.keep_last) / kGroup;
   if (rem > 0 && ng <= NTHR * 16 && static_cast<int>(rem) <= (last_beg - first_end) / 2) {
-    const int listed = ng <= NTHR * 3 ? find_groups<NTHR, 3>(sh, gmaxima, ng, rem, first_end, last_beg)
-                       : ng <= NTHR * 8
-                           ? find_groups<NTHR, 8>(sh, gmaxima, ng, rem, first_end, last_beg)
-                           : find_groups<NTHR, 16>(sh, gmaxima, ng, rem, first_end, last_beg);
+    unsigned bound;
+    const int listed =
+        ng <= NTHR * 3 ? find_groups<NTHR, 3>(sh, gmaxima, ng, rem, first_end, last_beg, bound)
+        : ng <= NTHR * 8
+            ? find_groups<NTHR, 8>(sh, gmaxima, ng, rem, first_end, last_beg, bound)
+            : find_groups<NTHR, 16>(sh, gmaxima, ng, rem, first_end, last_beg, bound);
     if (listed <= NTHR) {
+      // their keys that reach the bound, one a thread where they are few enough
       auto page = [&](int i) { return sh.groups[i / kGroup] * kGroup + i % kGroup; };
-      return choose_in_registers<NTHR, 8>(
-          sh, listed * kGroup, K, rem, [&](int i) { return key(page(i)); },
-          [&](int at, int i) { put(at, page(i)); });
+      KeyRegisters<NTHR, kGroup> k;
+      k.load(listed * kGroup, [&](int i) { return key(page(i)); });
+      const Before b = k.before(sh, bound - 1);
+      if (b.all_above <= NTHR) {
+        k.list(b, bound - 1, 0, [&](int at, int i, unsigned x) {
+          sh.key[at] = x;
+          sh.page[at] = page(i);
+        });
+        __syncthreads();
+        return choose_candidates<NTHR>(sh, static_cast<int>(b.all_above), K, rem, put);
+      }
     }
   }
   // all keys, read again for every bit
@@ -475,7 +517,8 @@ __device__ __forceinline__ void choose_pages(SelectShared<NTHR>& sh, const Selec
   Before b = block_before<NW>(sh, above, equal);
   const unsigned need = K - b.all_above;
   for (int i = beg; i < end; i += 32)
-    list_32(b, i + lane < end ? key(i + lane) : 0, thr, need, i + lane, put);
+    list_32(b, i + lane < end ? key(i + lane) : 0, thr, need, i + lane,
+            [&](int at, int j, unsigned) { put(at, j); });
 }
 
 // ---------------------------------------------------------------------------
