@@ -382,17 +382,6 @@ struct KeyRegisters {
   }
 };
 
-// put(place, i) for the K best of n places i in ascending order, `rem` of them not kForced.
-template <int NTHR, int J, typename Shared, typename Key, typename Put>
-__device__ __forceinline__ void choose_in_registers(Shared& sh, int n, unsigned K, unsigned rem,
-                                                    Key key, Put put) {
-  KeyRegisters<NTHR, J> r;
-  r.load(n, key);
-  const unsigned thr = rem > 0 ? r.threshold(sh, K, K) : kForced - 1;
-  const Before b = r.before(sh, thr);
-  r.list(b, thr, K - b.all_above, [&](int at, int i, unsigned) { put(at, i); });
-}
-
 // put(place, page) for the K best of n <= NTHR candidates in sh.key, one a thread, `rem` of
 // them not kForced: the barrier itself counts.
 template <int NTHR, typename Put>
@@ -419,6 +408,32 @@ __device__ __forceinline__ void choose_candidates(SelectShared<NTHR>& sh, int n,
   Before b = block_before<NW>(sh, k > thr, k == thr);
   list_32(b, k, thr, K - b.all_above, tid,
           [&](int at, int i, unsigned) { put(at, sh.page[i]); });
+}
+
+// put(place, i) for the K best of n places i in ascending order, `rem` of them not kForced.
+template <int NTHR, int J, typename Shared, typename Key, typename Put>
+__device__ __forceinline__ void choose_in_registers(Shared& sh, int n, unsigned K, unsigned rem,
+                                                    Key key, Put put) {
+  KeyRegisters<NTHR, J> r;
+  r.load(n, key);
+  unsigned thr = kForced - 1;
+  if constexpr (NTHR > 32) {
+    if (rem > 0 && K <= NTHR - NTHR / 8) {  // down to one candidate a thread first
+      thr = r.threshold(sh, K, NTHR) - 1;
+      const Before b = r.before(sh, thr);
+      if (b.all_above <= NTHR) {
+        r.list(b, thr, 0, [&](int at, int i, unsigned k) {
+          sh.key[at] = k;
+          sh.page[at] = i;
+        });
+        __syncthreads();
+        return choose_candidates<NTHR>(sh, static_cast<int>(b.all_above), K, rem, put);
+      }
+    }
+  }
+  if (rem > 0) thr = r.threshold(sh, K, K);
+  const Before b = r.before(sh, thr);
+  r.list(b, thr, K - b.all_above, [&](int at, int i, unsigned) { put(at, i); });
 }
 
 // The groups of 8 pages that matter into sh.groups: those whose largest open key reaches a
