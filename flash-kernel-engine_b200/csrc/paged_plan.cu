@@ -16,11 +16,12 @@
 // from the ring directly and not from the table, so no CTA reads what another one writes:
 // the ring's popped and pushed ranges are disjoint, and the only table entry a token reads
 // is the request's last, partly filled block. Rows of finished requests are read and
-// rewritten by one thread an entry. What bounds it is latency: the lengths' loads, the
+// rewritten by a warp. What bounds it is latency: the lengths' loads, the
 // sums (all loads first, then a contiguous range of requests a thread and one block-wide
 // scan of the ranges' sums), a binary search a token and the load of its block. 256 requests
-// of one token: 5.4 us a call; 4096 requests with 58 thousand tokens and 203 finished rows:
-// 10.4 us (24.6 us with the lengths loaded tile by tile and four tokens a thread).
+// of one token: 4.2 to 4.8 us a call; 4096 requests with 58 thousand tokens and 203 finished
+// rows: 9.1 us (24.6 us with the lengths loaded tile by tile and four tokens a thread, 11.3
+// with one entry of a finished row in flight a lane).
 #include <algorithm>
 
 #include "internal.h"
@@ -196,10 +197,22 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
       const int held = static_cast<int>(push[at(s + 1)] - push[at(s)]);
       const int now = (static_cast<int>(cu[at(s + 1)] - cu[at(s)]) + bs - 1) / bs;
       int* row = p.block_tables + static_cast<long long>(s) * p.width;
-      for (int j = lane; j < max(held, now); j += 32) {
-        const unsigned to = static_cast<unsigned>(count) + push[at(s)] + j;
-        if (j < held && to < static_cast<unsigned>(nb)) ring(to) = row[j];
-        if (j < now) row[j] = ring(pop[at(s)] + j);
+      // 8 entries a lane in flight: a long row's entries are one round trip, not one each
+      for (int j0 = lane; j0 < max(held, now); j0 += 256) {
+        int old[8], fresh[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int j = j0 + 32 * k;
+          if (j < held) old[k] = row[j];
+          if (j < now) fresh[k] = ring(pop[at(s)] + j);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int j = j0 + 32 * k;
+          const unsigned to = static_cast<unsigned>(count) + push[at(s)] + j;
+          if (j < held && to < static_cast<unsigned>(nb)) ring(to) = old[k];
+          if (j < now) row[j] = fresh[k];
+        }
       }
     }
   }
