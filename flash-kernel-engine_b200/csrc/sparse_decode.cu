@@ -117,6 +117,10 @@ struct Seq {
 __device__ __forceinline__ int pages_of(int ctx, int block_size) {
   return static_cast<int>((static_cast<long long>(ctx) + block_size - 1) / block_size);
 }
+// Pages of a sequence of `ctx` tokens within the table's width.
+__device__ __forceinline__ int pages_within(const SelectParams& p, int ctx) {
+  return min(pages_of(max(0, ctx), p.block_size), p.width);
+}
 __device__ __forceinline__ Seq seq_of(const SelectParams& p, int seq) {
   Seq r;
   r.ctx = max(0, __ldg(p.context_lens + seq));
@@ -135,14 +139,15 @@ __device__ __forceinline__ Seq seq_of(const SelectParams& p, int seq) {
 // query, the padding to 8 heads.
 template <typename T, int D>
 struct QueryHead {
-  static constexpr int E = D / 32;
-  float x[E];
+  static constexpr int PW = 4 / sizeof(T);  // channels a word
+  static constexpr int W = D / 32 / PW;     // words of a lane, 32 lanes side by side
+  uint32_t raw[W];
   bool real;
   __device__ __forceinline__ void load(const T* q) {  // nullptr: no query
     real = q != nullptr;
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(q);
 #pragma unroll
-    for (int i = 0; i < E; ++i)
-      x[i] = real ? static_cast<float>(q[i * 32 + (threadIdx.x & 31)]) : 0.f;
+    for (int i = 0; i < W; ++i) raw[i] = real ? __ldg(w + i * 32 + (threadIdx.x & 31)) : 0;
   }
   __device__ __forceinline__ void store(signed char* out, float2* scale) const {
     const int lane = threadIdx.x & 31;
@@ -153,12 +158,21 @@ struct QueryHead {
       if (lane == 0) *scale = make_float2(0.f, -kInf);
       return;
     }
-    float amax = 0.f;
+    float x[W][PW], amax = 0.f;
     bool fin = true;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      fin = fin && is_finite(x[i]);
-      amax = fmaxf(amax, fabsf(x[i]));
+    for (int i = 0; i < W; ++i) {
+      if constexpr (PW == 1) {
+        x[i][0] = __uint_as_float(raw[i]);
+      } else {
+        x[i][0] = static_cast<float>(reinterpret_cast<const T*>(&raw[i])[0]);
+        x[i][1] = static_cast<float>(reinterpret_cast<const T*>(&raw[i])[1]);
+      }
+#pragma unroll
+      for (int j = 0; j < PW; ++j) {
+        fin = fin && is_finite(x[i][j]);
+        amax = fmaxf(amax, fabsf(x[i][j]));
+      }
     }
     // non-negative floats are ordered as their bits
     amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
@@ -166,10 +180,14 @@ struct QueryHead {
     const int e = box_exponent(fin ? amax : 0.f);
     const float inv = exp2_int(-e);
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const int v = fin ? __float2int_rn(x[i] * inv) : 0;
-      out[i * 32 + lane] = static_cast<signed char>(max(v, 0));
-      out[D + i * 32 + lane] = static_cast<signed char>(min(v, 0));
+    for (int i = 0; i < W; ++i) {
+#pragma unroll
+      for (int j = 0; j < PW; ++j) {
+        const int at = (i * 32 + lane) * PW + j;
+        const int v = fin ? __float2int_rn(x[i][j] * inv) : 0;
+        out[at] = static_cast<signed char>(max(v, 0));
+        out[D + at] = static_cast<signed char>(min(v, 0));
+      }
     }
     if (lane == 0) *scale = fin ? make_float2(exp2_int(e), 0.f) : make_float2(0.f, kInf);
   }
@@ -578,8 +596,7 @@ __global__ void __launch_bounds__(32 * (kScoreWarps + 1), 1)
   // prefix sum of the tiles: a contiguous range of sequences a thread
   {
     auto count = [&](int i) {
-      const int pages =
-          min(pages_of(max(0, __ldg(p.context_lens + i)), p.block_size), p.width);
+      const int pages = pages_within(p, __ldg(p.context_lens + i));
       return pages > p.num_pages ? (pages + 15) / 16 : 0;
     };
     const int per = (p.num_seqs + NTH - 1) / NTH;
@@ -617,30 +634,41 @@ __global__ void __launch_bounds__(32 * (kScoreWarps + 1), 1)
     const int mid = (seq + hi) >> 1;
     if (pre[mid] <= at) seq = mid; else hi = mid;
   }
-  // block of a page (0 for one out of range: it is flagged where the page is listed)
-  auto block_of = [&](const Seq& r, int j) {
-    int b = 0;
-    if (j < r.pages) {
-      b = __ldg(r.table + j);
-      if (b < 0 || b >= p.num_blocks) b = 0;
-    }
-    return b;
-  };
   int slot = 0, phase = 0;  // of tile `at`
+  while (pre[seq + 1] <= at) ++seq;
+
+  // The table's entry for page j, looked at when it is used: nothing waits for a load that is
+  // for later. Past the sequence's pages it may be anything; an entry out of range counts as
+  // block 0 here (it is flagged where the page is listed).
+  auto entry = [&](int sq, int j) {
+    return j < p.width ? __ldg(p.block_tables + static_cast<long long>(sq) * p.width + j) : 0;
+  };
+  // the first of this CTA's boxes and scales of a block
+  auto box_of = [&](int b) {
+    return static_cast<long long>(b < 0 || b >= p.num_blocks ? 0 : b) * p.kv_heads + head0;
+  };
 
   if (warp == NW) {
     // ---- producer: two tiles a step, lanes 0..15 the first one's pages, the others the next
     const uint64_t policy = l2_policy_evict_first();
     const uint32_t bytes = nh * 2 * D;
-    while (at < stop) {
-      while (pre[seq + 1] <= at) ++seq;
-      const int t0 = at - pre[seq], t1 = min(stop, pre[seq + 1]) - pre[seq];
-      const Seq r = seq_of(p, seq);
-      auto blocks = [&](int t) { return t < t1 ? block_of(r, t * 16 + lane) : 0; };
-      int b0 = blocks(t0), b1 = blocks(t0 + 2), b2 = blocks(t0 + 4);
+    // for this lane's page of tiles t and t + 1
+    auto mine = [&](int sq, int t) { return entry(sq, t * 16 + lane); };
+    int t0 = at - pre[seq];
+    int b0 = mine(seq, t0), b1 = mine(seq, t0 + 2), b2 = mine(seq, t0 + 4);
+    while (true) {
+      const int t1 = min(stop, pre[seq + 1]) - pre[seq];
+      at += t1 - t0;
+      // the next sequence's first entries are on their way while this one's tiles are copied
+      int next = seq, n0 = 0, n1 = 0, n2 = 0;
+      if (at < stop) {
+        while (pre[next + 1] <= at) ++next;
+        n0 = mine(next, 0);
+        n1 = mine(next, 2);
+        n2 = mine(next, 4);
+      }
       for (int t = t0; t < t1; t += 2) {
-        const signed char* src =
-            p.values + (static_cast<long long>(b0) * p.kv_heads + head0) * (2 * D);
+        const signed char* src = p.values + box_of(b0) * (2 * D);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           if (t + k >= t1) break;
@@ -661,11 +689,15 @@ __global__ void __launch_bounds__(32 * (kScoreWarps + 1), 1)
         }
         b0 = b1;
         b1 = b2;
-        b2 = blocks(t + 6);
+        b2 = t + 6 < t1 ? mine(seq, t + 6) : 0;
       }
-      at += t1 - t0;
+      if (at >= stop) return;
+      seq = next;
+      t0 = 0;
+      b0 = n0;
+      b1 = n1;
+      b2 = n2;
     }
-    return;
   }
 
   // ---- consumers
@@ -689,26 +721,29 @@ __global__ void __launch_bounds__(32 * (kScoreWarps + 1), 1)
         if (i + k * NW < nh * GP) qh[k].store(rows + (i + k * NW) * 2 * D, scales + i + k * NW);
     }
   };
-  int buf = 0;
-  while (pre[seq + 1] <= at) ++seq;
-  query(seq, 0);
-  while (at < stop) {
-    while (pre[seq + 1] <= at) ++seq;
-    const int t0 = at - pre[seq], t1 = min(stop, pre[seq + 1]) - pre[seq];
-    const Seq r = seq_of(p, seq);
-    // this warp's first tile: its ring places are those with slot % step == group
-    const int skip = (group - slot % step + step) % step;
-    const int end = head < nh ? t1 : 0;
-    auto block_at = [&](int t) { return t < end ? block_of(r, t * 16 + page_at) : 0; };
-    auto scale_of = [&](int b) {
-      return __ldg(p.scales + static_cast<long long>(b) * p.kv_heads + head0 + min(head, nh - 1));
-    };
-    int b1 = block_at(t0 + skip), b2 = block_at(t0 + skip + step);
+  auto scale_of = [&](int b) { return __ldg(p.scales + box_of(b) + min(head, nh - 1)); };
+  // this warp's first tile: its ring places are those with slot % step == group
+  auto skip_at = [&](int slot) { return (group - slot % step + step) % step; };
+  int t0 = at - pre[seq], skip = skip_at(slot), ctx = __ldg(p.context_lens + seq);
+  int b1 = entry(seq, (t0 + skip) * 16 + page_at);
+  int b2 = entry(seq, (t0 + skip + step) * 16 + page_at);
+  for (int buf = 0;; buf ^= 1) {
+    const int t1 = min(stop, pre[seq + 1]) - pre[seq], n = slot + t1 - t0;
     float sc = scale_of(b1);
-    named_bar(1, NW * 32);  // this sequence's query rows are there
+    query(seq, buf);  // the other buffer was read before the last barrier but one
+    at += t1 - t0;
+    // the next sequence's length and first entries are on their way while this one is scored
+    int next = seq, next_ctx = 0, n1 = 0, n2 = 0;
+    const int next_skip = skip_at(n % stages);
+    if (at < stop) {
+      while (pre[next + 1] <= at) ++next;
+      next_ctx = __ldg(p.context_lens + next);
+      n1 = entry(next, next_skip * 16 + page_at);
+      n2 = entry(next, (next_skip + step) * 16 + page_at);
+    }
+    const int end = head < nh ? t1 : 0, pages = pages_within(p, ctx);
     const signed char* qr = qrow + (buf * head_group + head) * GP * 2 * D;
     const float2* qs = qscale + (buf * head_group + head) * GP;
-    buf ^= 1;
     const long long row = static_cast<long long>(seq) * p.kv_heads + head0 + head;
     unsigned* keys = p.keys + row * p.key_stride;
     unsigned* maxima = p.maxima + row * (p.key_stride / kGroup);
@@ -717,9 +752,10 @@ __global__ void __launch_bounds__(32 * (kScoreWarps + 1), 1)
       s -= stages;
       ++ph;
     }
+    named_bar(1, NW * 32);  // this sequence's query rows are there
     for (int t = t0 + skip; t < end; t += step) {
       const float sc_next = scale_of(b2);
-      b2 = block_at(t + 2 * step);
+      b2 = t + 2 * step < end ? entry(seq, (t + 2 * step) * 16 + page_at) : 0;
       const bool ok = __all_sync(
           0xffffffffu, *static_cast<volatile int*>(&dead) == 0 && mbar_wait(&full[s], ph & 1));
       if (!ok && lane == 0) {
@@ -727,7 +763,7 @@ __global__ void __launch_bounds__(32 * (kScoreWarps + 1), 1)
         atomicOr(p.err, kErrWaitTimeout);
       }
       if (ok) {
-        score_tile<D>(p, r.pages, ring + s * 16 * pitch + head * 2 * D, pitch, sc,
+        score_tile<D>(p, pages, ring + s * 16 * pitch + head * 2 * D, pitch, sc,
                       qr, qs, GP, t * 16, keys + t * 16, maxima + t * 2);
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[s]);
@@ -739,14 +775,15 @@ __global__ void __launch_bounds__(32 * (kScoreWarps + 1), 1)
         ++ph;
       }
     }
-    const int n = slot + t1 - t0;
+    if (at >= stop) return;
     slot = n % stages;
     phase += n / stages;
-    at += t1 - t0;
-    if (at < stop) {  // the next one's into the other buffer, read before the last barrier
-      while (pre[seq + 1] <= at) ++seq;
-      query(seq, buf);
-    }
+    seq = next;
+    ctx = next_ctx;
+    skip = next_skip;
+    t0 = 0;
+    b1 = n1;
+    b2 = n2;
   }
 }
 
