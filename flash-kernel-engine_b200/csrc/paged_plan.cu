@@ -53,6 +53,11 @@ __device__ __forceinline__ unsigned warp_scan_sat(unsigned v, int lane) {
 __device__ __forceinline__ int at(int s) { return s + (s >> 5); }
 __host__ __device__ constexpr int padded(int n) { return n + (n >> 5) + 1; }
 
+// ceil(n / d) without an overflow
+__device__ __forceinline__ unsigned ceil_div(unsigned n, unsigned d) {
+  return n == 0 ? 0 : (n - 1) / d + 1;
+}
+
 // Largest s in [0, S) with cu[s] <= t, for t < cu[S].
 __device__ __forceinline__ int request_of(const unsigned* cu, int S, unsigned t) {
   int lo = 0, hi = S;
@@ -95,13 +100,13 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     const int held = max(0, __ldg(p.context_lens + s)), add = max(0, __ldg(p.new_lens + s));
     const bool fin = finished(s);
     const int ctx = fin ? 0 : held;
-    const long long end = static_cast<long long>(ctx) + add;
-    const long long have = (static_cast<long long>(held) + bs - 1) / bs;
-    const long long need = (end + bs - 1) / bs - (fin ? 0 : have);
+    const unsigned end = static_cast<unsigned>(ctx) + static_cast<unsigned>(add);  // < 2^32
+    const unsigned have = ceil_div(held, bs);
+    const unsigned need = ceil_div(end, bs) - (fin ? 0 : have);
     // a request that its row cannot hold asks for more than there is
     cu[at(s + 1)] = end <= room ? min(add, kMaxPlanCount) : kMaxPlanCount;
-    pop[at(s + 1)] = static_cast<unsigned>(min(need, static_cast<long long>(kMaxPlanCount)));
-    push[at(s + 1)] = fin ? static_cast<unsigned>(min(have, static_cast<long long>(p.width))) : 0;
+    pop[at(s + 1)] = min(need, static_cast<unsigned>(kMaxPlanCount));
+    push[at(s + 1)] = fin ? min(have, static_cast<unsigned>(p.width)) : 0;
   }
   __syncthreads();
   // prefix sums: this thread's range, then the ranges before it

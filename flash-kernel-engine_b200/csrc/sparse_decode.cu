@@ -114,8 +114,8 @@ struct Seq {
   int ctx, pages;
   const int* table;
 };
-__device__ __forceinline__ int pages_of(int ctx, int block_size) {
-  return static_cast<int>((static_cast<long long>(ctx) + block_size - 1) / block_size);
+__device__ __forceinline__ int pages_of(int ctx, int block_size) {  // 16 or 32
+  return static_cast<int>((static_cast<unsigned>(ctx) + block_size - 1) >> (4 + (block_size >> 5)));
 }
 // Pages of a sequence of `ctx` tokens within the table's width.
 __device__ __forceinline__ int pages_within(const SelectParams& p, int ctx) {
@@ -625,8 +625,9 @@ __global__ void __launch_bounds__(32 * (kScoreWarps + 1), 1)
     __syncthreads();
   }
   const int total = pre[p.num_seqs];
-  int at = static_cast<int>(static_cast<long long>(total) * blockIdx.x / gridDim.x);
-  const int stop = static_cast<int>(static_cast<long long>(total) * (blockIdx.x + 1) / gridDim.x);
+  const unsigned each = static_cast<unsigned>(total) / gridDim.x, more = total - each * gridDim.x;
+  int at = each * blockIdx.x + min(blockIdx.x, more);
+  const int stop = at + each + (blockIdx.x < more ? 1 : 0);
   if (at >= stop) return;
   // the sequence of tile `at`: the last one that starts at or before it
   int seq = 0, hi = p.num_seqs;
@@ -1011,14 +1012,14 @@ __global__ void __launch_bounds__(NTHR, NT == 2 ? 1 : 512 / NTHR) sparse_decode_
   __syncthreads();
 
   // ---- this CTA's share of them
-  const int beg = static_cast<int>(static_cast<long long>(n) * rank / ctas);
-  const int end = static_cast<int>(static_cast<long long>(n) * (rank + 1) / ctas);
+  const int lg = 31 - __clz(ctas);  // ctas is a power of two, n at most kMaxFusedPages
+  const int beg = n * rank >> lg, end = n * (rank + 1) >> lg;
   const int spp = p.block_size / 16, pieces = (end - beg) * spp;
   const T* kc = static_cast<const T*>(p.k_cache);
   const T* vc = static_cast<const T*>(p.v_cache);
   // rows of piece u and the tokens in it
   auto locate = [&](int u, long long& at, int& limit) {
-    const int i = u / spp, half_ = u - i * spp;
+    const int i = u >> (spp >> 1), half_ = u - i * spp;  // spp is 1 or 2
     const int page = chosen[beg + i];
     const int b = __ldg(r.table + page);
     limit = r.ctx - page * p.block_size - half_ * 16;
