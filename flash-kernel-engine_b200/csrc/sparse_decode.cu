@@ -626,8 +626,10 @@ __global__ void __launch_bounds__(32 * (kScoreWarps + 1), 1)
   }
   const int total = pre[p.num_seqs];
   const unsigned each = static_cast<unsigned>(total) / gridDim.x, more = total - each * gridDim.x;
-  int at = each * blockIdx.x + min(blockIdx.x, more);
-  const int stop = at + each + (blockIdx.x < more ? 1 : 0);
+  // total * x / grid: where the sequences are equal and their number divides the grid, none
+  // of them changes inside a CTA's share
+  int at = each * blockIdx.x + more * blockIdx.x / gridDim.x;
+  const int stop = each * (blockIdx.x + 1) + more * (blockIdx.x + 1) / gridDim.x;
   if (at >= stop) return;
   // the sequence of tile `at`: the last one that starts at or before it
   int seq = 0, hi = p.num_seqs;
