@@ -18,11 +18,13 @@
 // paged_decode.cu.
 //
 // Choice. A score is kept as an ordered 32-bit key, with the largest key of every 8 pages.
-// Up to 8 pages a thread are held in registers, and the K-th largest key is found bit by bit
-// from the first bit in which the keys differ, one barrier a bit. Longer rows first look at
-// the groups' maxima in the same way: the m-th largest of them is a lower bound of the m-th
-// largest key, so that only keys that reach it matter: a few hundred of thousands, one a
-// thread. Where those are too many (equal scores, say), all keys are read again for every bit.
+// Up to 8 pages a thread are held in registers, and a threshold is found bit by bit from the
+// first bit in which the keys differ, one barrier a bit, until no more keys reach it than
+// there are threads; the K-th largest of those is then found with one key a thread, which
+// the barrier itself counts. Longer rows first look at the groups' maxima: the m-th largest
+// of them is a lower bound of the m-th largest key, so that only keys that reach it matter:
+// a few hundred of thousands. Where those are too many (equal scores, say), all keys are
+// read again for every bit.
 //
 // Two launches. page_score_kernel reads the boxes: one CTA an SM takes an equal share of all
 // sequences' 16-page tiles, whatever their lengths, and all KV heads of a tile at once, whose
@@ -562,10 +564,12 @@ __device__ __forceinline__ void choose_pages(SelectShared<NTHR>& sh, const Selec
 // a ring of tiles; consumer warp w scores head w % head_group of every (16 / head_group)th
 // tile. A tile's place in the ring always belongs to the same consumer warps (`stages` is a
 // multiple of 16 / head_group), so a parity wait cannot be satisfied by an older phase.
-// HBM bound once it streams: four contexts of 131072 tokens (67 MB of boxes) take 15 us, of
-// which 1.6 go to the prefix sum and 3 to the block table, the query and the first tiles;
-// then a CTA takes 46 GB/s, 6.8 TB/s in all. With the boxes read into registers, one row a
-// CTA, it took 20 us: 256-byte reads of one head at a time, and two tiles a warp in flight.
+// HBM bound once it streams: four contexts of 131072 tokens (67 MB of boxes) take 14 us, of
+// which 1.2 go to the prefix sum and 3 to the block table, the query and the first tiles;
+// then a CTA takes 46 GB/s, 6.8 TB/s in all. A change of the sequence inside a CTA's share
+// costs it 2 us, its query's (3.5 with its length, table and scales loaded only then). With
+// the boxes read into registers, one row a CTA, the launch took 20 us: 256-byte reads of one
+// head at a time, and two tiles a warp in flight.
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * (kScoreWarps + 1), 1)
     page_score_kernel(const SelectParams p, int head_group, int stages) {
@@ -970,9 +974,9 @@ struct SparseSmem {
   int chosen, got, total;
 };
 
-// Selection and attention of one (sequence, KV head) by a cluster of `ctas` CTAs. Of 26 us for
+// Selection and attention of one (sequence, KV head) by a cluster of `ctas` CTAs. Of 24 us for
 // four contexts of 131072 tokens and 256 pages (67 MB of keys and values), the choice takes
-// 7.5, the attention 13 (5 TB/s on 128 SMs) and the joins 2.7; 512 rows of 64 pages (268 MB)
+// 6.4, the attention 13 (5 TB/s on 128 SMs) and the joins 2.7; 512 rows of 64 pages (268 MB)
 // take 47 us in the attention, 5.7 TB/s.
 template <typename T, int D, int NT, int NTHR>
 __global__ void __launch_bounds__(NTHR, NT == 2 ? 1 : 512 / NTHR) sparse_decode_kernel(const SelectParams p, int ctas, const SparseSmem lay) {
@@ -1254,7 +1258,7 @@ static cudaError_t launch_d(SelectParams& p, bool fused, cudaStream_t st) {
         ctas *= 2;
       if (p.heads / p.kv_heads > 8) return launch_fused<T, D, 2, 256>(p, ctas, st);
       // more rows than SMs: four CTAs of 4 warps an SM, so that one's choice runs beside
-      // the others' copies (batch of 64 mixed contexts: 80 us; 90 us with two of 8 warps)
+      // the others' copies (batch of 64 mixed contexts: 76 us; 90 us with two of 8 warps)
       if (rows * ctas > sm_count()) return launch_fused<T, D, 1, 128>(p, ctas, st);
       return launch_fused<T, D, 1, 512>(p, ctas, st);
     }
