@@ -46,6 +46,7 @@
 
 #include "internal.h"
 #include "page_box.cuh"
+#include "page_key.h"
 #include "paged_decode.h"
 #include "paged_step.h"
 #include "ptx.cuh"
@@ -55,8 +56,6 @@ namespace cg = cooperative_groups;
 namespace fe {
 namespace step {
 
-constexpr unsigned kForced = 0xffffffffu;  // key of an always-chosen page, above every score
-constexpr float kInf = __builtin_huge_valf();
 constexpr int kMaxCtas = 8;            // of one (sequence, KV head): the portable cluster; of
                                        // clusters of 16 only four were resident at a time
 constexpr int kScoreWarps = 16;        // of a CTA of the score launch
@@ -65,12 +64,6 @@ constexpr int kScoreStages = 32;       // and tiles
 constexpr int kScoreSeqs = 4096;       // most sequences of one launch of it
 constexpr int kMaxFusedPages = 8192;   // most chosen pages whose list fits shared memory
 constexpr int kGroup = 8;              // pages whose largest key is kept
-
-// Order-preserving map of a float (no NaN, no -0) to 32 bits.
-__device__ __forceinline__ unsigned key_of(float x) {
-  const unsigned u = __float_as_uint(x);
-  return u ^ (static_cast<unsigned>(static_cast<int>(u) >> 31) | 0x80000000u);
-}
 
 // D = A(16x32, row) * B(32x8, col) + D, int8 inputs, int32 accumulate.
 __device__ __forceinline__ void mma_s8_16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -240,7 +233,7 @@ __device__ __forceinline__ void score_tile(const SelectParams& p, int pages,
   // lanes with an even cq have page gq, those with an odd one page gq + 8
   const int at = gq + 8 * (cq & 1), j = first + at;
   const float mine = cq & 1 ? best[1] : best[0];
-  unsigned key = key_of((sc == kInf ? sc : mine * sc) + 0.f);  // + 0: no -0
+  unsigned key = page_key(mine, sc);
   const bool in = j < pages, kept = j < p.keep_first || j >= pages - p.keep_last;
   unsigned open = in && !kept ? key : 0;
   key = !in ? 0 : kept ? kForced : key;

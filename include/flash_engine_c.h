@@ -456,7 +456,8 @@ int fe_update_page_bounds(const void* k_cache, signed char* values, float* scale
  * keep_first + keep_last. Boxes are read for full pages only that are neither the first
  * keep_first nor the last keep_last ones. q, caches, tables, lengths, scale, dtype,
  * kv_layout and the workspace are those of fe_paged_attention_ex; num_blocks must be
- * given, scale is positive. Outputs: out [S, H, d]; selected [S, Hkv, num_pages], the
+ * given, scale is positive. A page whose scale is NaN is ranked like one with the scale +inf.
+ * Outputs: out [S, H, d]; selected [S, Hkv, num_pages], the
  * chosen page indices in ascending order, -1 past their count. scratch:
  * fe_sparse_paged_attention_scratch_ints ints, any content. Two launches (scores, attention)
  * for bf16 / fp16 with the flat layout, at most 16 query heads a KV head and 8192 pages;
