@@ -74,6 +74,13 @@ double number(PyObject* o) {
 void same_device(const at::Tensor& a, const at::Tensor& b) {
   require(a.get_device() == b.get_device(), "all tensors must be on one device");
 }
+// Whether two contiguous tensors share memory.
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+  const char* x = static_cast<const char*>(a.data_ptr());
+  const char* y = static_cast<const char*>(b.data_ptr());
+  const size_t nx = a.nbytes(), ny = b.nbytes();
+  return nx > 0 && ny > 0 && x < y + ny && y < x + nx;
+}
 int dtype_code(at::ScalarType t) {
   return t == at::kBFloat16 ? 0 : t == at::kHalf ? 1 : t == at::kFloat ? 2 : -1;
 }
@@ -206,18 +213,25 @@ PyObject* plan(PyObject* const* a) {
   r[2].p = buffer(given[2], {cap}, at::kInt, ctx, "positions");
   r[3].p = buffer(given[3], {cap}, at::kLong, ctx, "slots");
   r[4].p = buffer(given[4], {4}, at::kInt, ctx, "free_state");
-  int* out_ctx = data<int>(THPVariable_Unpack(r[0].p));
-  int* out_state = data<int>(THPVariable_Unpack(r[4].p));
-  require((S == 0 || out_ctx != data<int>(ctx)) && out_state != data<int>(state),
-          "out must not hold inputs of the same call");
+  // every CTA reads all lengths while others write their share of the outputs
+  for (int i = 0; i < 5; ++i) {
+    const at::Tensor& o = THPVariable_Unpack(r[i].p);
+    for (const at::Tensor* t : {&ctx, &add, &table, &ring, &state})
+      require(!overlap(o, *t), "out must not hold inputs of the same call");
+    require(a[7] == Py_None || !overlap(o, THPVariable_Unpack(a[7])),
+            "out must not hold inputs of the same call");
+    for (int j = 0; j < i; ++j)
+      require(!overlap(o, THPVariable_Unpack(r[j].p)), "the tensors of out must not overlap");
+  }
   {
     const c10::cuda::OptionalCUDAGuard guard(ctx.device());
     check_status(c_plan(data<int>(ctx), data<int>(add), fin, data<int>(table), data<int>(ring),
-                        data<int>(state), out_ctx, data<int>(THPVariable_Unpack(r[1].p)),
+                        data<int>(state), data<int>(THPVariable_Unpack(r[0].p)),
+                        data<int>(THPVariable_Unpack(r[1].p)),
                         data<int>(THPVariable_Unpack(r[2].p)),
                         reinterpret_cast<long long*>(data<int64_t>(THPVariable_Unpack(r[3].p))),
-                        out_state, S, width, dim32(ring, 0), integer32(a[5]),
-                        static_cast<int>(cap), stream_of(ctx)),
+                        data<int>(THPVariable_Unpack(r[4].p)), S, width, dim32(ring, 0),
+                        integer32(a[5]), static_cast<int>(cap), stream_of(ctx)),
                  "plan_paged_step");
   }
   Ref t;

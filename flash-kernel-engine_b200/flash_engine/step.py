@@ -71,7 +71,8 @@ def plan_paged_step(context_lens, new_lens, block_tables, free_blocks, free_stat
     row; that one and those after it get no tokens (``free_state[2]`` counts the served
     ones). Tokens past the step's have position and slot -1, so that a step of fewer
     tokens runs with the same buffers. ``out``: the five tensors of a ``PagedStep`` to write
-    into (``max_tokens`` is then their length); they must not be inputs of this call."""
+    into (``max_tokens`` is then their length); they must share no memory with one another or
+    with the inputs of this call (ValueError)."""
     return PagedStep(*_native.plan(context_lens, new_lens, block_tables, free_blocks, free_state,
                                    block_size, max_tokens, finished, out))
 

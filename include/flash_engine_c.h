@@ -403,8 +403,8 @@ int fe_paged_decode_kv_range_nccl_bf16(const void* q, const void* k_cache, const
  *   positions [max_tokens]  position of each token in its request, -1 past the tokens
  *   slots [max_tokens]      block * block_size + offset, -1 past the tokens
  *   free_state_out [4]      (head, count, requests served, tokens)
- * block_tables and free_blocks are updated in place; context_lens_out may not be
- * context_lens, free_state_out may be neither free_state nor any other input. At most
+ * block_tables and free_blocks are updated in place; no other output may overlap an input or
+ * another output (not checked here). At most
  * 16384 requests; max_tokens and num_blocks below 2^30. A ring that would hold more than
  * num_blocks sets bit 1 of the device error word. */
 int fe_plan_paged_step(const int* context_lens, const int* new_lens,

@@ -29,3 +29,43 @@ def test_sparse_pages_with_nan_scales_rank_as_infinite_ones(dt, ctx):
         want = list(range(first)) + list(range(3, 3 + rest)) + list(range(pages - last, pages))
         assert got[0, 0].tolist() == want
         assert torch.isfinite(out).all() and fe().device_errors() == 0
+
+
+# ------------------------------------------------------------------------------- refusals
+def test_plan_refuses_outputs_that_share_memory_with_inputs_or_one_another():
+    """Some CTAs would read lengths that others have written over. Nothing is launched."""
+    S, cap = 6, 6
+    i32 = dict(dtype=torch.int32, device="cuda")
+    lens, new = torch.full((S,), 5, **i32), torch.ones(S, **i32)
+    table, ring = torch.zeros((S, 2), **i32), torch.arange(9, **i32)
+    state, finished = torch.tensor([0, 9, 0, 0], **i32), torch.zeros(S, dtype=torch.bool,
+                                                                     device="cuda")
+    out = lambda: [torch.empty(S, **i32), torch.empty(S + 1, **i32),  # noqa: E731
+                   torch.empty(cap, **i32), torch.empty(cap, dtype=torch.int64, device="cuda"),
+                   torch.empty(4, **i32)]
+    wide = torch.empty(64, **i32)  # outputs that overlap in part
+    part = [wide[:S], wide[S - 1:2 * S], wide[20:20 + cap], wide[28:28 + 2 * cap].view(torch.int64),
+            wide[60:]]
+    flags = torch.zeros(4 * S, dtype=torch.bool, device="cuda")
+    cases = [(0, lens), (0, new), (2, new), (2, lens), (4, state), (0, table.view(-1)[:S]),
+             (1, ring[:S + 1]), (4, ring[2:6]), (3, table.view(torch.int64).view(-1)),
+             (0, flags.view(torch.int32))]
+    before = [x.clone() for x in (lens, new, table, ring, state)]
+
+    def plan(o, fin=finished):
+        return fe().plan_paged_step(lens, new, table, ring, state, 16, finished=fin, out=tuple(o))
+
+    for k, t in cases:
+        o = out()
+        o[k] = t
+        with pytest.raises(ValueError, match="inputs"):
+            plan(o, flags[:S] if t.data_ptr() == flags.data_ptr() else finished)
+    for o in (part, (lambda o: [o[0], o[1], o[0], o[3], o[4]])(out())):
+        with pytest.raises(ValueError, match="overlap"):
+            plan(o)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(before, (lens, new, table, ring, state)))
+    # neighbours in one buffer share nothing
+    part[1] = wide[S:2 * S + 1]
+    assert plan(part).positions.tolist() == [5] * S
+    assert fe().device_errors() == 0
