@@ -18,6 +18,7 @@
 
 #include <climits>
 #include <cmath>
+#include <optional>
 #include <string>
 
 #include "../../include/flash_engine_c.h"
@@ -241,26 +242,38 @@ PyObject* plan(PyObject* const* a) {
   return t.release();
 }
 
-void run_bounds(const at::Tensor& k, PyObject* pair, const at::Tensor& slots, int block_size,
-                int layout) {
-  const int dt = dtype_code(k.scalar_type());
-  if (dt < 0) refuse(PyExc_TypeError, "unsupported dtype of key_cache");
-  const CacheDims c = cache_dims(k, block_size, layout);
-  const at::Tensor *values, *scales;
-  check_bounds(pair, c, k, &values, &scales);
-  require(slots.scalar_type() == at::kLong && slots.dim() == 1, "slots int64 [T] expected");
-  same_device(k, slots);
-  const c10::cuda::OptionalCUDAGuard guard(k.device());
-  check_status(c_bounds(k.data_ptr(), data<signed char>(*values), data<float>(*scales),
-                        reinterpret_cast<const long long*>(data<int64_t>(slots)),
-                        dim32(slots, 0), c.heads, c.dim, block_size, c.blocks, dt, layout,
-                        stream_of(k)),
-               "update_page_bounds");
-}
+// The arguments of the boxes' entry, checked; tokens = 0 asks the entry itself to check its own
+// and launch nothing.
+struct BoundsCall {
+  const at::Tensor *k, *values, *scales, *slots;
+  CacheDims c;
+  int block_size, dtype, layout;
+  BoundsCall(const at::Tensor& key_cache, PyObject* pair, const at::Tensor& slot_list, int bs,
+             int lay)
+      : k(&key_cache), slots(&slot_list), block_size(bs), dtype(dtype_code(key_cache.scalar_type())),
+        layout(lay) {
+    if (dtype < 0) refuse(PyExc_TypeError, "unsupported dtype of key_cache");
+    c = cache_dims(key_cache, bs, lay);
+    check_bounds(pair, c, key_cache, &values, &scales);
+    require(slot_list.scalar_type() == at::kLong && slot_list.dim() == 1,
+            "slots int64 [T] expected");
+    same_device(key_cache, slot_list);
+    run(0);
+  }
+  void run(int tokens) const {
+    const c10::cuda::OptionalCUDAGuard guard(k->device());
+    check_status(c_bounds(k->data_ptr(), data<signed char>(*values), data<float>(*scales),
+                          reinterpret_cast<const long long*>(data<int64_t>(*slots)), tokens,
+                          c.heads, c.dim, block_size, c.blocks, dtype, layout, stream_of(*k)),
+                 "update_page_bounds");
+  }
+};
 
 // (key_cache, page_bounds, slots, block_size, kv_layout)
 PyObject* bounds(PyObject* const* a) {
-  run_bounds(contiguous(a[0]), a[1], contiguous(a[2]), integer32(a[3]), layout_code(a[4]));
+  const at::Tensor& slots = contiguous(a[2]);
+  BoundsCall(contiguous(a[0]), a[1], slots, integer32(a[3]), layout_code(a[4]))
+      .run(dim32(slots, 0));
   Py_RETURN_NONE;
 }
 
@@ -324,6 +337,9 @@ PyObject* append(PyObject* const* a) {
   const int interleaved = PyObject_IsTrue(a[11]);
   if (interleaved < 0) throw Refusal{nullptr, {}};
   const double eps = number(a[9]);
+  // all that can be refused before the caches are written
+  std::optional<BoundsCall> boxes;
+  if (a[13] != Py_None) boxes.emplace(k, a[13], slots, bs, layout);
   Ref out;
   out.p = buffer(a[14], {T, heads, c.dim}, qkv.scalar_type(), qkv, "out");
   {
@@ -336,7 +352,7 @@ PyObject* append(PyObject* const* a) {
                  c.dim, bs, c.blocks, dt, layout, stream_of(qkv)),
         "paged_qkv_append");
   }
-  if (a[13] != Py_None) run_bounds(k, a[13], slots, bs, layout);
+  if (boxes) boxes->run(T);
   return out.release();
 }
 

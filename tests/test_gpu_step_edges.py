@@ -69,3 +69,33 @@ def test_plan_refuses_outputs_that_share_memory_with_inputs_or_one_another():
     part[1] = wide[S:2 * S + 1]
     assert plan(part).positions.tolist() == [5] * S
     assert fe().device_errors() == 0
+
+
+def test_append_refuses_page_bounds_before_it_writes():
+    """A call that is refused for its boxes has left queries and caches as they were."""
+    c, bf = dict(device="cuda"), dict(dtype=BF16, device="cuda")
+
+    def attempt(d, bs, bounds, error, Hkv=2, shift=0):
+        store = torch.zeros(4 * Hkv * bs * d + 8, **bf)
+        kc = store[shift:shift + 4 * Hkv * bs * d].view(4, Hkv, bs, d)
+        vc = torch.zeros((4, Hkv, bs, d), **bf)
+        q = torch.zeros((5, 4, d), **bf)
+        qkv = torch.randn((5, (4 + 2 * Hkv) * d), **c).to(BF16)
+        i = torch.arange(5, **c)
+        with pytest.raises(error):
+            fe().paged_qkv_append(qkv, kc, vc, i.int(), i, 4, bs, page_bounds=bounds, out=q)
+        torch.cuda.synchronize()
+        assert not kc.any() and not vc.any() and not q.any()
+
+    good = lambda d: fe().new_page_bounds(4, 2, d, "cuda")  # noqa: E731
+    b = good(64)
+    attempt(64, 16, (b.values[:, :1].contiguous(), b.scales), ValueError)
+    attempt(64, 16, (b.values, b.scales[:3]), ValueError)
+    attempt(64, 16, (b.values.int(), b.scales), ValueError)
+    attempt(64, 16, (b.values.transpose(1, 2), b.scales), ValueError)
+    attempt(64, 16, b.values, ValueError)
+    attempt(64, 16, (b.values.cpu(), b.scales), TypeError)
+    attempt(96, 16, good(96), RuntimeError)      # what the boxes do not take
+    attempt(64, 8, good(64), RuntimeError)
+    attempt(64, 16, good(64), RuntimeError, shift=4)
+    assert fe().device_errors() == 0
