@@ -383,10 +383,11 @@ PyObject* sparse(PyObject* const* a) {
   for (const at::Tensor* t : {&k, &v, &table, &lens}) same_device(q, *t);
   const at::Tensor *values, *scales;
   check_bounds(a[3], c, q, &values, &scales);
-  double scale = 1.0 / std::sqrt(static_cast<double>(c.dim));
+  float scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(c.dim)));
   if (a[8] != Py_None) {
-    scale = number(a[8]);
-    require(scale > 0, "scale must be positive");
+    // as the kernels take it: one that is 0 in fp32 would ask the entry for its default
+    scale = static_cast<float>(number(a[8]));
+    require(scale > 0, "scale must be positive in float32");
   }
   require(first >= 0 && last >= 1 && pages >= first + static_cast<long long>(last),
           "keep_first >= 0, keep_last >= 1 and num_pages >= their sum expected");
@@ -413,7 +414,7 @@ PyObject* sparse(PyObject* const* a) {
                  data<signed char>(*values), data<float>(*scales), data<int>(table),
                  data<int>(lens), data<int>(THPVariable_Unpack(sel.p)), data<int>(scratch), S, H,
                  c.heads, c.dim, bs, maxb, c.blocks, pages, first, last,
-                 static_cast<float>(scale), dt, layout, ws, ws_floats, stream_of(q)),
+                 scale, dt, layout, ws, ws_floats, stream_of(q)),
         "sparse_paged_attention");
   }
   Ref t;

@@ -118,7 +118,7 @@ def sparse_paged_attention(query, key_cache, value_cache, page_bounds, block_tab
                            workspace=None, out=None, selected=None):
     """Paged decode attention over ``num_pages`` pages of each (sequence, KV head).
 
-    ``query`` [S, H, d], caches, ``block_tables``, ``context_lens``, ``scale`` (positive)
+    ``query`` [S, H, d], caches, ``block_tables``, ``context_lens``, ``scale`` (positive in fp32)
     and ``workspace`` as for ``paged_attention`` (bf16, fp16, or fp32 with the flat layout;
     head_dim 64 or 128, block size 16 or 32). ``page_bounds``: the boxes of the full pages
     (``update_page_bounds``). Always attended: the first ``keep_first`` and the last

@@ -99,3 +99,19 @@ def test_append_refuses_page_bounds_before_it_writes():
     attempt(64, 8, good(64), RuntimeError)
     attempt(64, 16, good(64), RuntimeError, shift=4)
     assert fe().device_errors() == 0
+
+
+def test_sparse_scale_that_fp32_does_not_hold_is_refused():
+    """It would be 0 there, which the C entry takes as 1 / sqrt(d)."""
+    p = make_sparse(21, [60], 4, 2, 64, 16, BF16)
+    v, s = O.boxes(p["k"])
+    args = (cuda(p["q"], BF16), cuda(p["k"], BF16), cuda(p["v"], BF16), (cuda(v), cuda(s)),
+            cuda(p["tables"]), cuda(p["lens"]), 4, 16)
+    for scale in (1e-60, 0.0, -0.0, -1e-60, float("nan"), -1.0):
+        with pytest.raises(ValueError):
+            fe().sparse_paged_attention(*args, scale)
+    # the smallest ones that it does hold: equal weights, and not the default scale
+    tiny, _ = fe().sparse_paged_attention(*args, 2.0 ** -149)
+    assert torch.equal(tiny, fe().sparse_paged_attention(*args, 1e-30)[0])
+    assert not torch.equal(tiny, fe().sparse_paged_attention(*args)[0])
+    assert fe().device_errors() == 0
