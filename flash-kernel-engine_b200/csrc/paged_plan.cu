@@ -22,6 +22,8 @@
 // of one token: 4.2 to 4.8 us a call; 4096 requests with 58 thousand tokens and 203 finished
 // rows: 8.5 us (24.6 us with the lengths loaded tile by tile and four tokens a thread; 2.3
 // more with one entry of a finished row in flight a lane, 0.6 more with 64-bit divisions).
+#include <limits.h>
+
 #include <algorithm>
 
 #include "internal.h"
@@ -82,7 +84,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int head = max(0, __ldg(p.state)) % nb;
   const int count = min(max(0, __ldg(p.state + 1)), nb);
-  const long long room = static_cast<long long>(p.width) * bs;
+  // tokens a row can hold: its blocks', and a length has 31 bits
+  const unsigned room = static_cast<unsigned>(
+      min(static_cast<long long>(p.width) * bs, static_cast<long long>(INT_MAX)));
   auto finished = [&](int s) { return p.finished && p.finished[s]; };
   // ring entry head + k, k < 2^30
   auto ring = [&](unsigned k) -> int& {
@@ -162,7 +166,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
       const int s = request_of(cu, S, t);
       const bool fresh = finished(s);
       const int ctx = fresh ? 0 : max(0, __ldg(p.context_lens + s));
-      const int have = (ctx + bs - 1) / bs;
+      const int have = static_cast<int>(ceil_div(ctx, bs));
       pos = ctx + t - static_cast<int>(cu[at(s)]);
       const int j = pos / bs, off = pos - j * bs;
       int* entry = p.block_tables + static_cast<long long>(s) * p.width + j;
@@ -200,7 +204,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     for (int s = gtid >> 5; s < S; s += nth >> 5) {
       if (!p.finished[s]) continue;
       const int held = static_cast<int>(push[at(s + 1)] - push[at(s)]);
-      const int now = (static_cast<int>(cu[at(s + 1)] - cu[at(s)]) + bs - 1) / bs;
+      const int now = static_cast<int>(ceil_div(cu[at(s + 1)] - cu[at(s)], bs));
       int* row = p.block_tables + static_cast<long long>(s) * p.width;
       // 8 entries a lane in flight: a long row's entries are one round trip, not one each
       for (int j0 = lane; j0 < max(held, now); j0 += 256) {

@@ -396,8 +396,8 @@ int fe_paged_decode_kv_range_nccl_bf16(const void* q, const void* k_cache, const
  * blocks given back serve from the next step on). The free blocks are a ring:
  * free_blocks[(head + i) % num_blocks], i < count, free_state = (head, count).
  * Requests are served in order until one does not fit: its tokens in max_tokens, its
- * blocks in count, its length in max_blocks_per_seq * block_size. That one and every
- * later one get no tokens. Outputs:
+ * blocks in count, its length in max_blocks_per_seq * block_size and in 31 bits. That one
+ * and every later one get no tokens. Outputs:
  *   context_lens_out [S]    tokens held after the step
  *   cu_seqlens [S + 1]      first token of each request; cu_seqlens[S] = tokens
  *   positions [max_tokens]  position of each token in its request, -1 past the tokens

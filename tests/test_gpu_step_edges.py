@@ -115,3 +115,31 @@ def test_sparse_scale_that_fp32_does_not_hold_is_refused():
     assert torch.equal(tiny, fe().sparse_paged_attention(*args, 1e-30)[0])
     assert not torch.equal(tiny, fe().sparse_paged_attention(*args)[0])
     assert fe().device_errors() == 0
+
+
+# ------------------------------------------------------------ lengths near the end of 32 bits
+def test_plan_with_the_largest_blocks_and_lengths():
+    big = 2 ** 31 - 1
+    i = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+
+    def plan(ctx, new, tables, bs, finished=None, max_tokens=2):
+        t, ring = i(tables), i([0, 1, 2, 5])
+        s = fe().plan_paged_step(i(ctx), i(new), t, ring, i([0, 3]), bs, max_tokens=max_tokens,
+                                 finished=None if finished is None else
+                                 torch.tensor(finished, device="cuda"))
+        return [x.tolist() for x in s] + [t.tolist(), ring.tolist()]
+
+    # blocks of 2^31 - 1 tokens: the token goes to the row's own block
+    assert plan([2], [1], [[3]], big) == [[3], [0, 1], [2, -1], [3 * big + 2, -1], [0, 3, 1, 1],
+                                          [[3]], [0, 1, 2, 5]]
+    # a finished row of them gives its block back and takes a new one
+    assert plan([7], [2], [[3]], big, [True]) == [[2], [0, 2], [0, 1], [0, 1], [1, 3, 1, 2], [[0]],
+                                                  [0, 1, 2, 3]]
+    # a row with room for 2^31 tokens: a length ends at 2^31 - 1
+    assert plan([big - 1], [1], [[3, 2]], 2 ** 30) == [
+        [big], [0, 1], [big - 1, -1], [2 * 2 ** 30 + 2 ** 30 - 2, -1], [0, 3, 1, 1], [[3, 2]],
+        [0, 1, 2, 5]]
+    full = plan([big], [1], [[3, 2]], 2 ** 30)
+    assert full[0] == [big] and full[1] == [0, 0] and full[2] == [-1, -1]
+    assert full[4] == [0, 3, 0, 0] and full[5] == [[3, 2]]
+    assert fe().device_errors() == 0
