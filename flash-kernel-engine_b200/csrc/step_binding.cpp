@@ -75,12 +75,14 @@ double number(PyObject* o) {
 void same_device(const at::Tensor& a, const at::Tensor& b) {
   require(a.get_device() == b.get_device(), "all tensors must be on one device");
 }
-// Whether two contiguous tensors share memory.
+// Whether two ranges of bytes, or two contiguous tensors, share memory.
+bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
+  const char* x = static_cast<const char*>(a);
+  const char* y = static_cast<const char*>(b);
+  return na > 0 && nb > 0 && x < y + nb && y < x + na;
+}
 bool overlap(const at::Tensor& a, const at::Tensor& b) {
-  const char* x = static_cast<const char*>(a.data_ptr());
-  const char* y = static_cast<const char*>(b.data_ptr());
-  const size_t nx = a.nbytes(), ny = b.nbytes();
-  return nx > 0 && ny > 0 && x < y + ny && y < x + nx;
+  return overlap(a.data_ptr(), a.nbytes(), b.data_ptr(), b.nbytes());
 }
 int dtype_code(at::ScalarType t) {
   return t == at::kBFloat16 ? 0 : t == at::kHalf ? 1 : t == at::kFloat ? 2 : -1;
@@ -342,11 +344,19 @@ PyObject* append(PyObject* const* a) {
   if (a[13] != Py_None) boxes.emplace(k, a[13], slots, bs, layout);
   Ref out;
   out.p = buffer(a[14], {T, heads, c.dim}, qkv.scalar_type(), qkv, "out");
+  void* const out_at = THPVariable_Unpack(out.p).data_ptr();
+  void *const qkv_at = qkv.data_ptr(), *const k_at = k.data_ptr(), *const v_at = v.data_ptr();
+  if (a[14] != Py_None) {
+    const int64_t e = dt == 2 ? 4 : 2, n = e * T * heads * c.dim;
+    const int64_t cache = e * c.blocks * c.heads * bs * c.dim;
+    require(!overlap(out_at, n, qkv_at, e * ((T - 1) * stride + (heads + 2LL * c.heads) * c.dim)) &&
+                !overlap(out_at, n, k_at, cache) && !overlap(out_at, n, v_at, cache),
+            "out must not overlap qkv or the caches");
+  }
   {
     const c10::cuda::OptionalCUDAGuard guard(qkv.device());
     check_status(
-        c_append(qkv.data_ptr(), stride, THPVariable_Unpack(out.p).data_ptr(), k.data_ptr(),
-                 v.data_ptr(), data<int>(pos),
+        c_append(qkv_at, stride, out_at, k_at, v_at, data<int>(pos),
                  reinterpret_cast<const long long*>(data<int64_t>(slots)), w[0], w[1], wtype == 2,
                  static_cast<float>(eps), cos, sin, rotary, max_pos, interleaved, T, heads, c.heads,
                  c.dim, bs, c.blocks, dt, layout, stream_of(qkv)),

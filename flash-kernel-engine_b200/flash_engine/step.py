@@ -90,7 +90,8 @@ def paged_qkv_append(qkv, key_cache, value_cache, positions, slots, num_heads: i
     [T] (int32), pairs (2i, 2i + 1) if ``interleaved`` else (i, i + r / 2). Keys and values
     go to cache slots ``slots`` [T] (int64, block * block_size + offset); a negative slot is
     not cached, a negative position is padding (zero query row, nothing cached).
-    ``page_bounds``: also ``update_page_bounds`` of the pages this fills."""
+    ``page_bounds``: also ``update_page_bounds`` of the pages this fills. ``out`` may share no
+    memory with qkv or the caches (ValueError)."""
     return _native.append(qkv, key_cache, value_cache, positions, slots, num_heads, block_size,
                           q_weight, k_weight, eps, rope, interleaved, kv_layout, page_bounds, out)
 

@@ -143,3 +143,20 @@ def test_plan_with_the_largest_blocks_and_lengths():
     assert full[0] == [big] and full[1] == [0, 0] and full[2] == [-1, -1]
     assert full[4] == [0, 3, 0, 0] and full[5] == [[3, 2]]
     assert fe().device_errors() == 0
+
+
+def test_append_refuses_an_out_that_overlaps_qkv_or_the_caches():
+    T, H, Hkv, d, bs = 3, 4, 2, 64, 16
+    store = torch.zeros(4096 * 8, dtype=BF16, device="cuda")
+    wide = store[:T * 1000].view(T, 1000)
+    qkv = wide[:, :(H + 2 * Hkv) * d]
+    kc, vc = (store[at:at + 4 * Hkv * bs * d].view(4, Hkv, bs, d) for at in (8192, 20480))
+    i = torch.arange(T, device="cuda")
+    at = lambda x: store[x:x + T * H * d].view(T, H, d)  # noqa: E731
+    app = lambda out: fe().paged_qkv_append(qkv, kc, vc, i.int(), i, H, bs, out=out)  # noqa: E731
+    for x in (0, 2000, 2 * 1000 + (H + 2 * Hkv) * d - 1, 8192, 16000, 20480 - 1, 20480 + 8191):
+        with pytest.raises(ValueError, match="overlap"):
+            app(at(x))
+    for x in (2 * 1000 + (H + 2 * Hkv) * d, 16384, 20480 - T * H * d, 20480 + 8192):
+        app(at(x))
+    assert fe().device_errors() == 0
