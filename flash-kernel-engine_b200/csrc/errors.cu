@@ -5,6 +5,7 @@
 #include <stdio.h>
 
 #include "internal.h"
+#include "smem_optin.h"
 #include "../../include/flash_engine_c.h"
 
 namespace fe {
@@ -18,14 +19,6 @@ constexpr int kMaxDevices = 64;
 unsigned* g_err_ptr[kMaxDevices] = {};
 int g_sm_count[kMaxDevices] = {};
 std::mutex g_mu;
-
-struct SmemOptin {
-  const void* func;
-  int device;
-  int bytes;
-};
-SmemOptin g_optin[512];
-int g_n_optin = 0;
 
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 }  // namespace
@@ -62,18 +55,10 @@ int sm_count() {
 }
 
 cudaError_t ensure_smem_optin(const void* func, int bytes) {
-  const int d = current_device();
-  {
-    std::lock_guard<std::mutex> lk(g_mu);
-    for (int i = 0; i < g_n_optin; ++i)
-      if (g_optin[i].func == func && g_optin[i].device == d && g_optin[i].bytes >= bytes)
-        return cudaSuccess;
-  }
-  cudaError_t e = cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return e;
-  std::lock_guard<std::mutex> lk(g_mu);
-  if (g_n_optin < 512) g_optin[g_n_optin++] = SmemOptin{func, d, bytes};
-  return cudaSuccess;
+  static SmemOptin* const done = new SmemOptin;  // launches may come while statics are destroyed
+  return done->ensure(func, current_device(), bytes, [&](int n) {
+    return cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, n);
+  });
 }
 
 cudaError_t encode_tma_2d_b16(CUtensorMap* map, const void* base, bool bf16, uint64_t cols,

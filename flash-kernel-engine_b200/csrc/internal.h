@@ -1,7 +1,7 @@
 // Host-side helpers shared by the kernel files of libflash_engine_b200.so:
 // the device error word, cached device properties, the TMA descriptor encoder
 // (resolved through the runtime's driver entry point, so the library does not
-// link libcuda directly) and a one-time per-device smem opt-in.
+// link libcuda directly) and the opt-in of kernels to dynamic shared memory.
 #pragma once
 
 #include <cuda.h>
@@ -38,8 +38,8 @@ cudaError_t encode_tma_3d_b16(CUtensorMap* map, const void* base, bool bf16, uin
 cudaError_t encode_tma_3d_f32(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows,
                               uint64_t outer, uint32_t box_cols, uint32_t box_rows);
 
-// Calls cudaFuncSetAttribute(MaxDynamicSharedMemorySize) once per
-// (function, device).
+// Raises a kernel's MaxDynamicSharedMemorySize on the current device to `bytes`, unless an
+// earlier call has done so (smem_optin.h).
 cudaError_t ensure_smem_optin(const void* func, int bytes);
 
 inline cudaError_t stream_ok(void* stream) {

@@ -61,3 +61,59 @@ def test_keys_are_in_the_order_of_the_scores(page_key):
     assert page_key.key(-0.0, 1.0) == page_key.key(0.0, 1.0)
     for sc, best in ((inf, -5.0), (inf, 0.0), (nan, 1.0), (nan, -1.0), (-inf, 0.0), (0.0, inf)):
         assert page_key.key(best, sc) == keys[-1], (sc, best)
+
+
+# ----------------------------------------------------------- the shared memory of the kernels
+def test_shared_memory_opt_in_never_shrinks(tmp_path):
+    """Threads that launch kernels of changing sizes: at each launch the attribute (the last
+    value set) covers what it needs, and a kernel's sizes take one record however many."""
+    run = host_library(tmp_path, '''
+        #include "smem_optin.h"
+        #include <atomic>
+        #include <thread>
+        #include <vector>
+        // Returns launches that would fail; calls[0] counts the sets.
+        extern "C" int run(int threads, int rounds, int kernels, int fail_every, int* calls) {
+          fe::SmemOptin optin;
+          std::vector<std::atomic<int>> attribute(kernels);
+          for (auto& a : attribute) a = 48 * 1024;
+          std::atomic<int> bad{0}, sets{0};
+          std::vector<std::thread> all;
+          for (int t = 0; t < threads; ++t)
+            all.emplace_back([&, t] {
+              unsigned x = 12345u + 777u * t;
+              for (int i = 0; i < rounds; ++i) {
+                x = x * 1664525u + 1013904223u;
+                const int k = (x >> 8) % kernels, bytes = 50000 + (x >> 12) % 150000;
+                const int e = optin.ensure(&attribute[k], 0, bytes, [&](int n) {
+                  const int at = ++sets;
+                  if (fail_every && at % fail_every == 0) return 1;
+                  std::this_thread::yield();
+                  attribute[k] = n;
+                  return 0;
+                });
+                if (e == 0 && attribute[k] < bytes) ++bad;
+              }
+            });
+          for (auto& t : all) t.join();
+          calls[0] = sets;
+          return bad;
+        }
+        extern "C" int devices() {  // one function on two devices: two records
+          fe::SmemOptin optin;
+          int n = 0, f = 0;
+          auto set = [&](int) { ++n; return 0; };
+          optin.ensure(&f, 0, 100, set);
+          optin.ensure(&f, 1, 100, set);
+          optin.ensure(&f, 0, 100, set);
+          optin.ensure(&f, 1, 90, set);
+          optin.ensure(&f, 1, 101, set);
+          return n;
+        }''')
+    calls = ctypes.c_int()
+    for fail_every in (0, 7):
+        for kernels in (1, 3, 700):
+            assert run.run(8, 20000, kernels, fail_every, ctypes.byref(calls)) == 0
+            # running maxima of random sizes: a few sets a kernel
+            assert calls.value < 40 * kernels + (20 if fail_every else 0)
+    assert run.devices() == 3
