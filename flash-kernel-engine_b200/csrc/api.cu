@@ -561,7 +561,9 @@ int fe_paged_qkv_append(const void* qkv, long long row_stride, void* q_out, void
   p.weight_f32 = weight_fp32;
   p.kv_layout = kv_layout;
   p.err = err;
-  return static_cast<int>(fe::step::launch_qkv_append(p, dtype, as_stream(stream)));
+  const cudaError_t e = fe::step::launch_qkv_append(p, dtype, as_stream(stream));
+  if (e == cudaSuccess) fe::tables_passed(as_stream(stream));  // it waits for a plan before it
+  return static_cast<int>(e);
 }
 
 int fe_update_page_bounds(const void* k_cache, signed char* values, float* scales,
@@ -578,7 +580,9 @@ int fe_update_page_bounds(const void* k_cache, signed char* values, float* scale
   if (!err) return static_cast<int>(cudaErrorInitializationError);
   const fe::step::BoundsParams p{k_cache, values, scales, slots, T, Hkv, num_blocks, kv_layout,
                                  err};
-  return static_cast<int>(fe::step::launch_page_bounds(p, d, bs, dtype, as_stream(stream)));
+  const cudaError_t e = fe::step::launch_page_bounds(p, d, bs, dtype, as_stream(stream));
+  if (e == cudaSuccess) fe::tables_passed(as_stream(stream));
+  return static_cast<int>(e);
 }
 
 int fe_sparse_paged_attention(const void* q, const void* kc, const void* vc, void* out,
@@ -648,6 +652,7 @@ int fe_sparse_paged_attention(const void* q, const void* kc, const void* vc, voi
   sp.err = err;
   const bool fused = fe::step::sparse_fused(sp, dtype, kv_layout);
   const cudaError_t e = fe::step::launch_sparse(sp, d, dtype, fused, st);
+  if (e == cudaSuccess) fe::tables_passed(st);  // the decode of the other form has a.serial
   if (e != cudaSuccess || fused) return static_cast<int>(e);
   if (dtype == 0)
     return lib ? paged_v1_entry<__nv_bfloat16>(a, st)

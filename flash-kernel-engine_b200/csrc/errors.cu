@@ -5,6 +5,7 @@
 #include <stdio.h>
 
 #include "internal.h"
+#include "launch_order.h"
 #include "smem_optin.h"
 #include "../../include/flash_engine_c.h"
 
@@ -60,6 +61,13 @@ cudaError_t ensure_smem_optin(const void* func, int bytes) {
     return cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, n);
   });
 }
+
+static TableWriters& table_writers() {
+  static TableWriters* const w = new TableWriters;
+  return *w;
+}
+void tables_written(cudaStream_t stream) { table_writers().wrote(current_device(), stream); }
+bool tables_passed(cudaStream_t stream) { return table_writers().passed(current_device(), stream); }
 
 cudaError_t encode_tma_2d_b16(CUtensorMap* map, const void* base, bool bf16, uint64_t cols,
                               uint64_t rows, uint64_t row_stride_elems, uint32_t box_cols,

@@ -42,6 +42,12 @@ cudaError_t encode_tma_3d_f32(CUtensorMap* map, const void* base, uint64_t cols,
 // earlier call has done so (smem_optin.h).
 cudaError_t ensure_smem_optin(const void* func, int bytes);
 
+// Bookkeeping of launch_order.h on the current device: a kernel that writes block tables or
+// lengths was launched on the stream; one was behind which they are sure to be seen (returns
+// whether the stream ended in a writer).
+void tables_written(cudaStream_t stream);
+bool tables_passed(cudaStream_t stream);
+
 inline cudaError_t stream_ok(void* stream) {
   (void)stream;
   return cudaSuccess;

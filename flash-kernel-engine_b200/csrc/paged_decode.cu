@@ -540,10 +540,12 @@ __global__ void __maxnreg__((DecodeRegs<T, NT>::value))
     part_ml = part_o + static_cast<size_t>(gridDim.x) * 2 * HPC * D;
   }
 
-  // Until griddepcontrol.wait below, this grid touches only shared memory and the two
-  // inputs that no kernel of this library writes, context_lens and block_tables: the
-  // prefix over the sequences and the producer's first block-table group are read
-  // while the previous grid (typically the previous decode step) is still finishing.
+  // Until griddepcontrol.wait below, this grid touches only shared memory and two inputs,
+  // context_lens and block_tables: the prefix over the sequences and the producer's first
+  // block-table group are read while the previous grid (typically the previous decode
+  // step) is still finishing. Where the previous kernel is one of this library's that
+  // writes them (the step plan, the page selection), this grid is launched without
+  // programmatic serialization and starts after it (launch_order.h).
   // This grid can start before the previous kernel in the stream has completed only if
   // that kernel executed griddepcontrol.launch_dependents, which only this library's
   // kernels do; inputs written by a copy, a host write or any kernel that does not
@@ -1541,7 +1543,8 @@ static cudaError_t launch_cfg(const Params& p, const void* kc, const void* vc, l
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = p.serial ? 0 : 1;
+  const bool after_writer = tables_passed(stream);
+  cfg.numAttrs = p.serial || after_writer ? 0 : 1;
   return cudaLaunchKernelEx(&cfg, kern, km, vm, pp);
 }
 

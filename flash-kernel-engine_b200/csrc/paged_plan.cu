@@ -239,13 +239,14 @@ cudaError_t launch_plan(const PlanParams& p, cudaStream_t stream) {
   cfg.blockDim = dim3(kPlanThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  // placed while the kernel before finishes (it waits for it), and not triggering itself:
-  // the decode reads lengths and tables before its own wait
+  // placed while the kernel before finishes (it waits for it); a decode that comes next reads
+  // lengths and tables before its own wait, and is told to start after this kernel
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  tables_written(stream);
   return cudaLaunchKernelEx(&cfg, plan_kernel, p);
 }
 

@@ -160,3 +160,65 @@ def test_append_refuses_an_out_that_overlaps_qkv_or_the_caches():
     for x in (2 * 1000 + (H + 2 * Hkv) * d, 16384, 20480 - T * H * d, 20480 + 8192):
         app(at(x))
     assert fe().device_errors() == 0
+
+
+# ------------------------------------------------------------------- launches right in a row
+@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("between", [False, True])
+def test_dense_decode_right_behind_the_plan(dt, between):
+    """plan -> dense decode -> plan -> .. on one stream with nothing between them (or with an
+    append and a sparse attention): every decode attends to the lengths and tables of its
+    own step."""
+    from oracle import attention_oracle as A
+    bs, S, H, Hkv, d, nb, width, steps = 16, 7, 8, 2, 64, 160, 16, 12
+    g = np.random.default_rng(5)
+    k, v = (torch.from_numpy(g.standard_normal((nb, Hkv, bs, d))).cuda().to(dt) for _ in range(2))
+    q = [torch.from_numpy(g.standard_normal((S, H, d))).cuda().to(dt) for _ in range(steps)]
+    new = g.integers(1, 20, (steps, S)).astype(np.int32)
+    new[0] = g.integers(1, 60, S)
+    fin = g.random((steps, S)) < 0.25
+    fin[0] = False
+    cap = int(new.sum(1).max())
+    qkv = torch.randn((cap, (H + 2 * Hkv) * d), device="cuda").to(dt)
+    pb = fe().new_page_bounds(nb, Hkv, d, "cuda")
+    dnew, dfin = [cuda(x) for x in new], [cuda(x) for x in fin]
+    tables, ring = cuda(np.zeros((S, width), np.int32)), cuda(np.arange(nb, dtype=np.int32))
+    lens, state = cuda(np.zeros(S, np.int32)), cuda(np.array([3, nb, 0, 0], np.int32))
+    kw = dict(dtype=torch.int32, device="cuda")
+    bufs = [(torch.empty(S, **kw), torch.empty(S + 1, **kw), torch.empty(cap, **kw),
+             torch.empty(cap, dtype=torch.int64, device="cuda"), torch.empty(4, **kw))
+            for _ in range(steps)]
+    outs = [torch.empty_like(x) for x in q]
+    # what each step's decode reads: its own lengths and tables, and the caches as they are then
+    want, m_tables, m_ring, m_state = [], np.zeros((S, width), np.int32), ring.cpu().numpy(), [3, nb]
+    m_lens = np.zeros(S, int)
+    for i in range(steps):
+        r = O.plan(m_lens, new[i], m_tables, m_ring, m_state[0], m_state[1], bs, cap, fin[i])
+        assert r["state"][2] == S
+        m_lens, m_tables, m_ring = r["context_lens"].astype(int), r["tables"], r["ring"]
+        m_state = [int(r["state"][0]), int(r["state"][1])]
+        want.append((m_tables, m_lens.astype(np.int32), r["positions"], r["slots"]))
+    caches = [(k.clone(), v.clone())]
+    if between:
+        for i in range(steps - 1):
+            kk, vv = (x.clone() for x in caches[-1])
+            fe().paged_qkv_append(qkv, kk, vv, cuda(want[i][2]), cuda(want[i][3]), H, bs)
+            caches.append((kk, vv))
+    torch.cuda.synchronize()
+    for i in range(steps):
+        s = fe().plan_paged_step(lens, dnew[i], tables, ring, state, bs, finished=dfin[i],
+                                 out=bufs[i])
+        fe().paged_attention(q[i], k, v, tables, s.context_lens, bs, out=outs[i])
+        if between:
+            fe().paged_qkv_append(qkv, k, v, s.positions, s.slots, H, bs, page_bounds=pb)
+            fe().sparse_paged_attention(q[i], k, v, pb, tables, s.context_lens, 3, bs)
+        lens, state = s.context_lens, s.free_state
+    torch.cuda.synchronize()
+    f64 = lambda x: x.double().cpu().numpy()  # noqa: E731
+    for i in range(steps):
+        kk, vv = caches[i if between else 0]
+        ref = A.paged_attention_gqa(f64(q[i]), f64(kk), f64(vv), want[i][0], want[i][1])
+        err = np.abs(f64(outs[i]) - ref).max()
+        assert err <= (2e-2 if dt == BF16 else 1e-3), (i, err)
+    np.testing.assert_array_equal(tables.cpu().numpy(), want[-1][0])
+    assert fe().device_errors() == 0

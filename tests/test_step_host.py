@@ -1,5 +1,5 @@
 """Host-side parts of the serving-step operators, compiled into small host programs: the keys
-that pages are chosen by."""
+that pages are chosen by, the kernels' shared memory, the order of launches."""
 import ctypes
 import os
 import shutil
@@ -117,3 +117,43 @@ def test_shared_memory_opt_in_never_shrinks(tmp_path):
             # running maxima of random sizes: a few sets a kernel
             assert calls.value < 40 * kernels + (20 if fail_every else 0)
     assert run.devices() == 3
+
+
+# -------------------------------------------------------------------- the order of the launches
+def test_a_decode_right_behind_a_writer_of_tables_starts_after_it(tmp_path):
+    lib = host_library(tmp_path, '''
+        #include "launch_order.h"
+        #include <thread>
+        static fe::TableWriters w;
+        extern "C" void wrote(int d, long s) { w.wrote(d, reinterpret_cast<void*>(s)); }
+        extern "C" int passed(int d, long s) { return w.passed(d, reinterpret_cast<void*>(s)); }
+        // Threads with a stream each: every decode after a plan has to see it.
+        extern "C" int race(int threads, int rounds) {
+          fe::TableWriters x;
+          std::vector<std::thread> all;
+          std::atomic<int> bad{0};
+          for (long t = 0; t < threads; ++t)
+            all.emplace_back([&, t] {
+              const void* s = reinterpret_cast<const void*>(t);
+              for (int i = 0; i < rounds; ++i) {
+                x.wrote(0, s);
+                if (i & 1) x.wrote(0, s);
+                bad += !x.passed(0, s);
+                bad += x.passed(0, s);
+              }
+            });
+          for (auto& t : all) t.join();
+          return bad;
+        }''')
+    lib.wrote.argtypes = lib.passed.argtypes = [ctypes.c_int, ctypes.c_long]
+    assert not lib.passed(0, 0)                      # nothing written yet
+    lib.wrote(0, 0)                                  # plan -> decode -> decode
+    assert lib.passed(0, 0) and not lib.passed(0, 0)
+    lib.wrote(0, 7)                                  # another stream, another device
+    assert not lib.passed(0, 0) and not lib.passed(1, 7)
+    lib.wrote(0, 0)
+    lib.wrote(0, 0)
+    lib.wrote(1, 0)
+    assert lib.passed(0, 0) and not lib.passed(0, 0)
+    assert lib.passed(0, 7) and lib.passed(1, 0) and not lib.passed(1, 0)
+    assert lib.race(8, 20000) == 0
