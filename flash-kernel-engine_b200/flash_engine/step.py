@@ -24,17 +24,25 @@ import torch
 from . import _lib
 from .ops import _workspace
 
-try:
-    from . import _step_native as _native
-except ImportError as e:
-    raise ImportError(
-        f"the native binding {os.path.join(os.path.dirname(__file__), '_step_native.so')} cannot "
-        "be loaded; build it with `make -C flash-kernel-engine_b200/csrc` (or "
-        f"__graft_entry__.build()): {e}") from e
+_native = None
 
-_native.bind(*(ctypes.cast(getattr(_lib.lib, n), ctypes.c_void_p).value for n in (
-    "fe_plan_paged_step", "fe_paged_qkv_append", "fe_update_page_bounds",
-    "fe_sparse_paged_attention", "fe_sparse_paged_attention_scratch_ints")))
+
+def _load():
+    """The native binding, loaded when the first of these operators is called: the others of
+    the package do without it."""
+    global _native
+    try:
+        from . import _step_native as native
+    except ImportError as e:
+        raise ImportError(
+            f"the native binding _step_native of {os.path.dirname(__file__)} cannot be loaded; "
+            "build it with `make -C flash-kernel-engine_b200/csrc` (or "
+            f"__graft_entry__.build()): {e}") from e
+    native.bind(*(ctypes.cast(getattr(_lib.lib, n), ctypes.c_void_p).value for n in (
+        "fe_plan_paged_step", "fe_paged_qkv_append", "fe_update_page_bounds",
+        "fe_sparse_paged_attention", "fe_sparse_paged_attention_scratch_ints")))
+    _native = native
+    return native
 
 
 class PagedStep(NamedTuple):
@@ -73,8 +81,9 @@ def plan_paged_step(context_lens, new_lens, block_tables, free_blocks, free_stat
     tokens runs with the same buffers. ``out``: the five tensors of a ``PagedStep`` to write
     into (``max_tokens`` is then their length); they must share no memory with one another or
     with the inputs of this call (ValueError)."""
-    return PagedStep(*_native.plan(context_lens, new_lens, block_tables, free_blocks, free_state,
-                                   block_size, max_tokens, finished, out))
+    native = _native or _load()
+    return PagedStep(*native.plan(context_lens, new_lens, block_tables, free_blocks, free_state,
+                                  block_size, max_tokens, finished, out))
 
 
 def paged_qkv_append(qkv, key_cache, value_cache, positions, slots, num_heads: int,
@@ -92,8 +101,9 @@ def paged_qkv_append(qkv, key_cache, value_cache, positions, slots, num_heads: i
     not cached, a negative position is padding (zero query row, nothing cached).
     ``page_bounds``: also ``update_page_bounds`` of the pages this fills. ``out`` may share no
     memory with qkv or the caches (ValueError)."""
-    return _native.append(qkv, key_cache, value_cache, positions, slots, num_heads, block_size,
-                          q_weight, k_weight, eps, rope, interleaved, kv_layout, page_bounds, out)
+    native = _native or _load()
+    return native.append(qkv, key_cache, value_cache, positions, slots, num_heads, block_size,
+                         q_weight, k_weight, eps, rope, interleaved, kv_layout, page_bounds, out)
 
 
 def new_page_bounds(num_blocks: int, num_kv_heads: int, head_dim: int, device) -> PageBounds:
@@ -109,7 +119,7 @@ def update_page_bounds(key_cache, page_bounds, slots, block_size: int = 16, *,
     page's last place; others are skipped), read from the cache. Call it after the step's
     keys are in the cache, with the step's slots. head_dim 64 or 128, block size 16 or 32.
     Returns page_bounds."""
-    _native.bounds(key_cache, page_bounds, slots, block_size, kv_layout)
+    (_native or _load()).bounds(key_cache, page_bounds, slots, block_size, kv_layout)
     return page_bounds
 
 
@@ -128,11 +138,12 @@ def sparse_paged_attention(query, key_cache, value_cache, page_bounds, block_tab
     exact whole-number arithmetic, so the choice depends on the inputs alone. Sequences of
     at most ``num_pages`` pages are attended whole. Returns (out [S, H, d], selected
     [S, Hkv, num_pages] int32: the pages in ascending order, -1 past their count)."""
+    native = _native or _load()
     if workspace is not None or not _fused(query, key_cache, num_pages, kv_layout):
         workspace = _decode_workspace(query, key_cache, block_size, workspace)
-    return _native.sparse(query, key_cache, value_cache, page_bounds, block_tables, context_lens,
-                          num_pages, block_size, scale, keep_first, keep_last, kv_layout,
-                          workspace, out, selected)
+    return native.sparse(query, key_cache, value_cache, page_bounds, block_tables, context_lens,
+                         num_pages, block_size, scale, keep_first, keep_last, kv_layout,
+                         workspace, out, selected)
 
 
 def _fused(query, key_cache, num_pages, kv_layout):

@@ -4,6 +4,7 @@ import ctypes
 import os
 import shutil
 import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -157,3 +158,39 @@ def test_a_decode_right_behind_a_writer_of_tables_starts_after_it(tmp_path):
     assert lib.passed(0, 0) and not lib.passed(0, 0)
     assert lib.passed(0, 7) and lib.passed(1, 0) and not lib.passed(1, 0)
     assert lib.race(8, 20000) == 0
+
+
+# ------------------------------------------------------------------------- the native binding
+def test_package_works_without_the_native_binding():
+    """Only the serving-step operators need it, and they say what is missing when called."""
+    code = '''
+import sys
+class Absent:
+    def find_spec(self, name, path=None, target=None):
+        if name.endswith("_step_native"):
+            raise ImportError("not built")
+sys.meta_path.insert(0, Absent())
+import torch, flash_engine as F
+z = torch.zeros(1)
+for call in (lambda: F.paged_attention(z, z, z, z, z), lambda: F.flash_attention(z, z, z)):
+    try:
+        call()
+    except TypeError:
+        pass
+    else:
+        raise AssertionError
+F.new_page_bounds(2, 1, 64, "cpu")
+for call in (lambda: F.plan_paged_step(z, z, z, z, z, max_tokens=4),
+             lambda: F.paged_qkv_append(z, z, z, z, z, 4),
+             lambda: F.update_page_bounds(z, (z, z), z),
+             lambda: F.sparse_paged_attention(z, z, z, (z, z), z, z, 4)):
+    try:
+        call()
+    except ImportError as e:
+        assert "make -C" in str(e) and "not built" in str(e), e
+    else:
+        raise AssertionError
+'''
+    r = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, PYTHONPATH=PKG),
+                       capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
