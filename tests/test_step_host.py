@@ -5,6 +5,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 import numpy as np
 import pytest
@@ -165,6 +166,7 @@ def test_package_works_without_the_native_binding():
     """Only the serving-step operators need it, and they say what is missing when called."""
     code = '''
 import sys
+import sysconfig
 class Absent:
     def find_spec(self, name, path=None, target=None):
         if name.endswith("_step_native"):
@@ -194,3 +196,40 @@ for call in (lambda: F.plan_paged_step(z, z, z, z, z, max_tokens=4),
     r = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, PYTHONPATH=PKG),
                        capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
+
+
+def make(*args):
+    r = subprocess.run(["make", "-C", CSRC, *args], capture_output=True, text=True)
+    return r.returncode, r.stdout + r.stderr
+
+
+@pytest.mark.skipif(shutil.which("make") is None, reason="needs make")
+def test_library_builds_without_torch(tmp_path):
+    """Dry runs into an empty folder, with an interpreter that has no torch."""
+    to = (f"OBJDIR={tmp_path}/obj", f"OUTDIR={tmp_path}/lib", "PYTHON=false")
+    for goal in ((), ("lib",)):
+        rc, out = make("-n", *to, *goal)
+        assert rc == 0 and "libflash_engine_b200.so" in out and "step_binding.cpp" not in out
+    rc, out = make(*to, "binding")
+    assert rc != 0 and "torch" in out
+
+
+@pytest.mark.skipif(shutil.which("make") is None, reason="needs make")
+def test_binding_is_built_again_for_another_interpreter_or_torch(tmp_path):
+    binding, stamp = tmp_path / "native.so", tmp_path / "obj" / "binding.stamp"
+    to = (f"OBJDIR={tmp_path}/obj", f"PYTHON={sys.executable}", "binding")
+    as_named, given = to, to + (f"BINDING={binding}",)
+    rc, out = make("-n", *as_named)
+    suffix = sysconfig.get_config_var("EXT_SUFFIX")
+    assert rc == 0 and (f"_step_native{suffix} " in out or "up to date" in out or
+                        "Nothing to be done" in out)
+    rc, out = make("-n", *given)
+    assert rc == 0 and "step_binding.cpp" in out      # not there yet
+    binding.touch()
+    rc, out = make("-n", *given)
+    assert rc == 0 and "step_binding.cpp" not in out  # newer than all it comes from
+    stamp.write_text("another torch\n")
+    past = binding.stat().st_mtime - 100
+    os.utime(stamp, (past, past))
+    rc, out = make("-n", *given)
+    assert rc == 0 and "step_binding.cpp" in out
