@@ -5,7 +5,9 @@ import pytest
 import torch
 
 from gpu_util import cuda
-from test_gpu_step import BF16, F16, F32, O, fe, make_sparse
+from step_util import attention_bound
+from test_gpu_step import BF16, F16, F32, O, fe, make_sparse, vllm_k, vllm_v
+from test_step_tolerance import LONG
 
 pytestmark = pytest.mark.gpu
 
@@ -222,3 +224,40 @@ def test_dense_decode_right_behind_the_plan(dt, between):
         assert err <= (2e-2 if dt == BF16 else 1e-3), (i, err)
     np.testing.assert_array_equal(tables.cpu().numpy(), want[-1][0])
     assert fe().device_errors() == 0
+
+
+# ------------------------------------------------- outputs, to within what their sums allow
+def check_outputs(p, num_pages, first=1, last=1, layout="flat"):
+    """Chosen pages equal, every output within the bound of step_util.py."""
+    v, s = O.boxes(p["k"])
+    S, Hkv, G = len(p["lens"]), p["k"].shape[1], p["q"].shape[1] // p["k"].shape[1]
+    sel = np.full((S, Hkv, num_pages), -1, np.int32)
+    for i in range(S):
+        for h in range(Hkv):
+            pages = O.select(p["q"][i, h * G:(h + 1) * G], v[:, h], s[:, h], p["tables"][i],
+                             p["lens"][i], p["bs"], num_pages, first, last)
+            sel[i, h, :len(pages)] = pages
+    dt, vl = p["dt"], layout == "vllm"
+    out, got = fe().sparse_paged_attention(
+        cuda(p["q"], dt), cuda(vllm_k(p["k"]) if vl else p["k"], dt),
+        cuda(vllm_v(p["v"]) if vl else p["v"], dt), (cuda(v), cuda(s)), cuda(p["tables"]),
+        cuda(p["lens"]), num_pages, p["bs"], keep_first=first, keep_last=last, kv_layout=layout)
+    np.testing.assert_array_equal(got.cpu().numpy(), sel)
+    ref, bound = attention_bound(p, sel)
+    over = np.abs(out.double().cpu().numpy() - ref) / np.maximum(bound, 1e-300)
+    assert (over <= 1).all(), float(over.max())
+    assert fe().device_errors() == 0
+
+
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
+@pytest.mark.parametrize("case", LONG, ids=lambda c: f"{c[1][0]}-{c[6]}")
+def test_sparse_outputs_of_many_pages(case, dt):
+    """A CTA's share, a join weight or the end of the list lost would show (see
+    test_step_tolerance.py)."""
+    check_outputs(make_sparse(*case[:6], dt), case[6])
+
+
+@pytest.mark.parametrize("layout", ["flat", "vllm"])
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_sparse_outputs_of_many_pages_in_both_layouts(dt, layout):
+    check_outputs(make_sparse(34, [9000, 5000], 8, 2, 64, 16, dt), 200, layout=layout)
