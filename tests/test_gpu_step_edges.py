@@ -261,3 +261,19 @@ def test_sparse_outputs_of_many_pages(case, dt):
 @pytest.mark.parametrize("dt", [BF16, F16])
 def test_sparse_outputs_of_many_pages_in_both_layouts(dt, layout):
     check_outputs(make_sparse(34, [9000, 5000], 8, 2, 64, 16, dt), 200, layout=layout)
+
+
+@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("H,Hkv,d,bs", [
+    (9, 9, 64, 16), (12, 12, 128, 16), (32, 32, 128, 16), (40, 40, 64, 32),  # one head a group
+    (64, 16, 64, 16), (80, 10, 128, 16),                                     # and more
+    (64, 4, 128, 16), (48, 3, 128, 32), (128, 8, 128, 16),  # query rows that shrink the group
+    (80, 2, 128, 16), (130, 2, 64, 16)])                    # more heads than a fused call takes
+def test_sparse_more_kv_heads_than_a_score_cta_takes(dt, H, Hkv, d, bs):
+    """The scores of several groups of KV heads, the last one not full."""
+    check_outputs(make_sparse(H + Hkv, [700, 31, 1500, 0, 6 * bs + 1], H, Hkv, d, bs, dt), 6)
+
+
+@pytest.mark.parametrize("H,Hkv", [(9, 9), (64, 16)])
+def test_sparse_more_kv_heads_over_long_rows(H, Hkv):
+    check_outputs(make_sparse(40 + Hkv, [20000, 3001], H, Hkv, 64, 16, BF16), 40, 2, 3)
