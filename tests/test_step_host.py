@@ -23,7 +23,7 @@ def host_library(tmp_path, source, *flags):
     src, out = tmp_path / "host.cpp", tmp_path / "host.so"
     src.write_text(source)
     subprocess.run(["g++", "-std=c++17", "-O2", "-Wall", "-shared", "-fPIC", "-pthread",
-                    f"-I{CSRC}", f"-I{CUDA}/include", *flags, "-o", str(out), str(src)], check=True)
+                    f"-I{CSRC}", f"-I{CUDA}/include", "-o", str(out), str(src), *flags], check=True)
     return ctypes.CDLL(str(out))
 
 
@@ -233,3 +233,73 @@ def test_binding_is_built_again_for_another_interpreter_or_torch(tmp_path):
     os.utime(stamp, (past, past))
     rc, out = make("-n", *given)
     assert rc == 0 and "step_binding.cpp" in out
+
+
+# ------------------------------------------------------------------------- the C++ launchers
+def test_cpp_launchers_pass_their_arguments_in_order(tmp_path):
+    """serving_step.cuh against the library: what each launcher refuses, one field at a time
+    (nothing is launched: no tokens, no sequences)."""
+    lib = os.path.join(PKG, "flash_engine", "lib")
+    if not os.path.exists(os.path.join(lib, "libflash_engine_b200.so")):
+        pytest.skip("the library is not built")
+    source = '''
+        #include "serving_step.cuh"
+        using namespace flash_engine::serving;
+        static char at[64] __attribute__((aligned(64)));
+        template <typename T> T* p() { return reinterpret_cast<T*>(at); }
+        static int plan(StepPlanConfig c) {  // no outputs: refused by then if all else is right
+          return launch_plan_paged_step(p<int>(), p<int>(), nullptr, p<int>(), p<int>(), p<int>(),
+                                        p<int>(), p<int>(), p<int>(), p<long long>(), nullptr, c);
+        }
+        static int append(int tokens, int heads, long long stride, CacheConfig c, float eps = 0,
+                          RopeTables r = {}) {
+          return launch_paged_qkv_append(p<void>(), stride, p<void>(), p<void>(), p<void>(),
+                                         p<int>(), p<long long>(), nullptr, nullptr, false, eps, r,
+                                         tokens, heads, c);
+        }
+        static int bounds(int tokens, CacheConfig c) {
+          return launch_update_page_bounds(p<void>(), p<signed char>(), p<float>(),
+                                           p<long long>(), tokens, c);
+        }
+        static int sparse(int seqs, int heads, int width, int pages, int first, int last,
+                          CacheConfig c) {
+          return launch_sparse_paged_attention(
+              p<void>(), p<void>(), p<void>(), p<void>(), p<signed char>(), p<float>(), p<int>(),
+              p<int>(), p<int>(), p<int>(), seqs, heads, width, pages, first, last, 0.1f, c);
+        }
+        extern "C" int run() {
+          const CacheConfig c{4, 2, 64, 16};
+          const int bad = cudaErrorInvalidValue;
+          int n = 0;  // the first check that fails
+        #define CHECK(x) ++n; if (!(x)) return n;
+          CHECK(plan({1, 2, 8, 16, 4}) == bad)
+          CHECK(append(0, 4, 512, c) == 0)
+          CHECK(append(0, 4, 511, c) == bad)
+          CHECK(append(0, 0, 512, c) == bad)
+          CHECK(append(-1, 4, 512, c) == bad)
+          CHECK(append(0, 4, 512, c, -1.f) == bad)
+          RopeTables r{p<float>(), p<float>(), 64, 8, true};
+          CHECK(append(0, 4, 512, c, 0.f, r) == 0)
+          r.rotary_dim = 66;
+          CHECK(append(0, 4, 512, c, 0.f, r) == bad)
+          r.rotary_dim = 64;
+          r.max_pos = 0;
+          CHECK(append(0, 4, 512, c, 0.f, r) == bad)
+          CHECK(append(0, 4, 512, {4, 2, 64, 16, DType::kFp32, KvLayout::kVllm}) == bad)
+          CHECK(append(0, 4, 512, {4, 2, 64, 16, DType::kFp32}) == 0)
+          CHECK(bounds(0, c) == 0 && bounds(-1, c) == bad)
+          CHECK(bounds(0, {4, 2, 96, 16}) == bad && bounds(0, {4, 2, 64, 8}) == bad)
+          CHECK(bounds(0, {0, 2, 64, 16}) == bad && bounds(0, {4, 0, 64, 16}) == bad)
+          CHECK(bounds(0, {4, 2, 128, 32}) == 0)
+          CHECK(sparse(0, 4, 8, 3, 1, 2, c) == 0)
+          CHECK(sparse(0, 4, 8, 3, 1, 3, c) == bad)
+          CHECK(sparse(0, 4, 8, 3, 2, 0, c) == bad)
+          CHECK(sparse(0, 5, 8, 3, 1, 2, c) == bad)
+          CHECK(sparse(0, 4, 0, 3, 1, 2, c) == bad)
+          CHECK(sparse(-1, 4, 8, 3, 1, 2, c) == bad)
+          CHECK(sparse(0, 4, 8, 3, 1, 2, {4, 2, 64, 32, DType::kBf16, KvLayout::kVllm}) == bad)
+          return 0;
+        }'''
+    include = os.path.join(os.path.dirname(PKG), "include")
+    assert host_library(tmp_path, source, f"-I{include}", f"-L{lib}", f"-Wl,-rpath,{lib}",
+                        "-l:libflash_engine_b200.so").run() == 0
