@@ -5,12 +5,13 @@
 * ``paged_qkv_append``       -- per-head QK norm, rotary embedding and cache write of the
   step's tokens in one pass over their QKV projection;
 * ``update_page_bounds``     -- int8 boxes of the keys of the pages the step filled;
-* ``sparse_paged_attention`` -- decode attention over the pages whose boxes bound q.k
-  highest.
+* ``sparse_paged_attention`` -- decode attention over the pages whose boxes score highest
+  for the query.
 
-Everything stays on the GPU and on the current stream: no call synchronises, and with
-``out=`` buffers none allocates anything a CUDA graph could not keep. As in ``ops``, inputs
-must be CUDA tensors (TypeError otherwise) and unsupported shapes raise.
+Everything stays on the GPU and on the current stream: no call synchronises, and all can be
+captured in a CUDA graph. With ``out=`` buffers the first three allocate nothing; the sparse
+attention takes its scratch (the scores) from torch's allocator at every call. As in ``ops``,
+inputs must be CUDA tensors (TypeError otherwise) and unsupported shapes raise.
 """
 
 from __future__ import annotations
@@ -133,10 +134,15 @@ def sparse_paged_attention(query, key_cache, value_cache, page_bounds, block_tab
     and ``workspace`` as for ``paged_attention`` (bf16, fp16, or fp32 with the flat layout;
     head_dim 64 or 128, block size 16 or 32). ``page_bounds``: the boxes of the full pages
     (``update_page_bounds``). Always attended: the first ``keep_first`` and the last
-    ``keep_last`` (>= 1) pages; the rest of ``num_pages`` are those whose box bounds the
-    largest q.k of the group's query heads highest, ties to the lower page. The scores are
-    exact whole-number arithmetic, so the choice depends on the inputs alone. Sequences of
-    at most ``num_pages`` pages are attended whole. Returns (out [S, H, d], selected
+    ``keep_last`` (>= 1) pages; the rest of ``num_pages`` are those with the highest scores,
+    ties to the lower page. A page's score is the largest product that a key inside its box
+    could have with a query head of the group, each head rounded to 8-bit whole numbers and a
+    power of two: near an upper bound of the page's q.k, above or below it by the rounding of
+    the query, and loose where one channel's keys are far larger than the others', which share
+    its exponent. The scores are exact whole-number arithmetic, so the choice depends on the
+    inputs alone. Sequences of at most ``num_pages`` pages are attended whole. bf16 and fp16
+    round the softmax weights to 16 bits for the product with V, as ``paged_attention`` does.
+    Returns (out [S, H, d], selected
     [S, Hkv, num_pages] int32: the pages in ascending order, -1 past their count)."""
     native = _native or _load()
     if workspace is not None or not _fused(query, key_cache, num_pages, kv_layout):

@@ -450,16 +450,17 @@ int fe_update_page_bounds(const void* k_cache, signed char* values, float* scale
                           void* stream);
 
 /* Paged decode attention over num_pages pages of each (sequence, KV head): the first
- * keep_first and the last keep_last (>= 1) pages and those whose boxes bound q.k highest
- * (over the group's query heads; the query rounded to whole numbers like a box; ties to
- * the lower page). A sequence of at most num_pages pages is attended whole. num_pages >=
+ * keep_first and the last keep_last (>= 1) pages and those with the highest scores: the
+ * largest product that a key inside the page's box could have with a query head of the
+ * group, the head rounded to nearest whole numbers of at most 127 and a power of two; ties
+ * go to the lower page. A sequence of at most num_pages pages is attended whole. num_pages >=
  * keep_first + keep_last. Boxes are read for full pages only that are neither the first
  * keep_first nor the last keep_last ones. q, caches, tables, lengths, scale, dtype,
  * kv_layout and the workspace are those of fe_paged_attention_ex; num_blocks must be
- * given, scale is positive. A page whose scale is NaN is ranked like one with the scale +inf.
- * Outputs: out [S, H, d]; selected [S, Hkv, num_pages], the
- * chosen page indices in ascending order, -1 past their count. scratch:
- * fe_sparse_paged_attention_scratch_ints ints, any content. Two launches (scores, attention)
+ * given, scale is positive. A page whose scale is NaN is ranked like one with the scale
+ * +inf. Outputs: out [S, H, d]; selected [S, Hkv, num_pages], the chosen page indices in
+ * ascending order, -1 past their count. scratch: fe_sparse_paged_attention_scratch_ints
+ * ints, any content. Two launches (scores, attention)
  * for bf16 / fp16 with the flat layout, at most 16 query heads a KV head and 8192 pages;
  * otherwise scores, selection and the decode of fe_paged_attention_ex with a block table for
  * each (sequence, KV head), which alone uses the workspace. */
