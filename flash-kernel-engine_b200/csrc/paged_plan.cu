@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
       const int s = request_of(cu, S, t);
       const bool fresh = finished(s);
       const int ctx = fresh ? 0 : max(0, __ldg(p.context_lens + s));
-      const int have = static_cast<int>(ceil_div(ctx, bs));
+      const int have = static_cast<int>((static_cast<unsigned>(ctx) + bs - 1u) / bs);  // < 2^32
       pos = ctx + t - static_cast<int>(cu[at(s)]);
       const int j = pos / bs, off = pos - j * bs;
       int* entry = p.block_tables + static_cast<long long>(s) * p.width + j;
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     for (int s = gtid >> 5; s < S; s += nth >> 5) {
       if (!p.finished[s]) continue;
       const int held = static_cast<int>(push[at(s + 1)] - push[at(s)]);
-      const int now = static_cast<int>(ceil_div(cu[at(s + 1)] - cu[at(s)], bs));
+      const int now = static_cast<int>((cu[at(s + 1)] - cu[at(s)] + bs - 1u) / bs);  // < 2^32
       int* row = p.block_tables + static_cast<long long>(s) * p.width;
       // 8 entries a lane in flight: a long row's entries are one round trip, not one each
       for (int j0 = lane; j0 < max(held, now); j0 += 256) {
