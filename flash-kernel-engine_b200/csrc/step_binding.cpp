@@ -319,8 +319,8 @@ PyObject* append(PyObject* const* a) {
   }
   const float *cos = nullptr, *sin = nullptr;
   int rotary = 0, max_pos = 0;
+  Ref seq;  // until the launch: the tables of an iterator have no other owner
   if (a[10] != Py_None) {
-    Ref seq;
     seq.p = PySequence_Tuple(a[10]);
     if (!seq.p) throw Refusal{nullptr, {}};
     require(PyTuple_GET_SIZE(seq.p) == 2, "rope must be (cos, sin)");

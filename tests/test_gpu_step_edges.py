@@ -277,3 +277,25 @@ def test_sparse_more_kv_heads_than_a_score_cta_takes(dt, H, Hkv, d, bs):
 @pytest.mark.parametrize("H,Hkv", [(9, 9), (64, 16)])
 def test_sparse_more_kv_heads_over_long_rows(H, Hkv):
     check_outputs(make_sparse(40 + Hkv, [20000, 3001], H, Hkv, 64, 16, BF16), 40, 2, 3)
+
+
+# --------------------------------------------------------------- arguments made for the call
+@pytest.mark.parametrize("T", [64, 1024])
+def test_append_with_rope_tables_that_live_as_long_as_the_call(T):
+    """rope may be any pair, an iterator of fresh tensors too: the queries' memory must not be
+    that of a table that was let go before the kernel ran."""
+    H, Hkv, d, bs = 8, 2, 128, 16
+    g = torch.Generator(device="cuda").manual_seed(1)
+    qkv = torch.randn((T, (H + 2 * Hkv) * d), device="cuda", generator=g).to(BF16)
+    angle = torch.rand((T * H, d // 2), device="cuda", generator=g)  # a table like out
+    tables = [angle.cos(), angle.sin()]
+    pos = torch.arange(T, dtype=torch.int32, device="cuda")
+    slots = torch.arange(T, device="cuda")
+    cache = lambda: torch.zeros((T // bs, Hkv, bs, d), dtype=BF16, device="cuda")  # noqa: E731
+    app = lambda rope: fe().paged_qkv_append(qkv, cache(), cache(), pos, slots, H, bs,  # noqa: E731
+                                             rope=rope)
+    want = app(tuple(tables))
+    assert tables[0].nbytes == want.nbytes
+    for _ in range(20):
+        assert torch.equal(app(x.clone() for x in tables), want)
+    assert torch.equal(app(tables), want)
