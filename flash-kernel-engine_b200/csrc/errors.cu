@@ -2,6 +2,7 @@
 #include <cudaTypedefs.h>
 
 #include <mutex>
+#include <new>
 #include <stdio.h>
 
 #include "internal.h"
@@ -22,6 +23,15 @@ int g_sm_count[kMaxDevices] = {};
 std::mutex g_mu;
 
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
+
+// The library's one T, never destroyed: launches may come while statics are. In static storage,
+// so that nothing is allocated for it.
+template <typename T>
+T& lasting() {
+  alignas(T) static unsigned char at[sizeof(T)];
+  static T* const t = new (at) T;
+  return *t;
+}
 }  // namespace
 
 int current_device() {
@@ -56,18 +66,20 @@ int sm_count() {
 }
 
 cudaError_t ensure_smem_optin(const void* func, int bytes) {
-  static SmemOptin* const done = new SmemOptin;  // launches may come while statics are destroyed
-  return done->ensure(func, current_device(), bytes, [&](int n) {
-    return cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, n);
-  });
+  return lasting<SmemOptin>().ensure(
+      func, current_device(), bytes,
+      [&](int n) {
+        return cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, n);
+      },
+      cudaErrorMemoryAllocation);
 }
 
-static TableWriters& table_writers() {
-  static TableWriters* const w = new TableWriters;
-  return *w;
+void tables_written(cudaStream_t stream) {
+  lasting<TableWriters>().wrote(current_device(), stream);
 }
-void tables_written(cudaStream_t stream) { table_writers().wrote(current_device(), stream); }
-bool tables_passed(cudaStream_t stream) { return table_writers().passed(current_device(), stream); }
+bool tables_passed(cudaStream_t stream) {
+  return lasting<TableWriters>().passed(current_device(), stream);
+}
 
 cudaError_t encode_tma_2d_b16(CUtensorMap* map, const void* base, bool bf16, uint64_t cols,
                               uint64_t rows, uint64_t row_stride_elems, uint32_t box_cols,

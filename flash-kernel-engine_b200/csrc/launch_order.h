@@ -19,16 +19,24 @@ namespace fe {
 
 class TableWriters {
  public:
-  // A kernel that writes tables or lengths goes on the stream.
-  void wrote(int device, const void* stream) {
+  // A kernel that writes tables or lengths goes on the stream. These are called from C entries:
+  // nothing is thrown, and where a stream cannot be recorded every stream counts as one that
+  // ends in a writer from then on.
+  void wrote(int device, const void* stream) noexcept {
     std::lock_guard<std::mutex> lk(mu_);
-    if (find(device, stream) == last_.end()) last_.emplace_back(device, stream);
-    count_ = static_cast<int>(last_.size());
+    if (find(device, stream) != last_.end()) return;
+    try {
+      last_.emplace_back(device, stream);
+      count_ = static_cast<int>(last_.size());
+    } catch (...) {
+      all_ = true;
+    }
   }
   // A kernel goes on the stream behind which the tables are sure to be seen. Returns whether
   // the stream ended in a writer.
-  bool passed(int device, const void* stream) {
-    if (count_.load() == 0) return false;
+  bool passed(int device, const void* stream) noexcept {
+    if (all_) return true;
+    if (count_ == 0) return false;
     std::lock_guard<std::mutex> lk(mu_);
     const auto it = find(device, stream);
     if (it == last_.end()) return false;
@@ -45,6 +53,7 @@ class TableWriters {
   }
   std::mutex mu_;
   std::atomic<int> count_{0};  // a call with no writer anywhere takes no lock
+  std::atomic<bool> all_{false};
   std::vector<Stream> last_;
 };
 

@@ -15,14 +15,20 @@ namespace fe {
 // launch of 150 KB would fail.
 class SmemOptin {
  public:
-  // set(bytes): raises the attribute; 0 on success. Returns its result, or 0 without a call.
-  template <typename Set>
-  auto ensure(const void* func, int device, int bytes, Set set) -> decltype(set(bytes)) {
+  // set(bytes): raises the attribute; 0 on success. Returns its result, 0 without a call, or
+  // no_memory where there is none for a record (called from C entries: nothing is thrown).
+  template <typename Set, typename Error>
+  Error ensure(const void* func, int device, int bytes, Set set, Error no_memory) noexcept {
     std::lock_guard<std::mutex> lk(mu_);
-    const auto it = bytes_.try_emplace(std::make_pair(func, device), 0).first;
-    if (it->second >= bytes) return {};
-    const auto e = set(bytes);
-    if (e == decltype(e){}) it->second = bytes;
+    int* have = nullptr;
+    try {
+      have = &bytes_[std::make_pair(func, device)];
+    } catch (...) {
+      return no_memory;
+    }
+    if (*have >= bytes) return Error{};
+    const Error e = set(bytes);
+    if (e == Error{}) *have = bytes;
     return e;
   }
 

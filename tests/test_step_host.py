@@ -93,7 +93,7 @@ def test_shared_memory_opt_in_never_shrinks(tmp_path):
                   std::this_thread::yield();
                   attribute[k] = n;
                   return 0;
-                });
+                }, 2);
                 if (e == 0 && attribute[k] < bytes) ++bad;
               }
             });
@@ -105,11 +105,9 @@ def test_shared_memory_opt_in_never_shrinks(tmp_path):
           fe::SmemOptin optin;
           int n = 0, f = 0;
           auto set = [&](int) { ++n; return 0; };
-          optin.ensure(&f, 0, 100, set);
-          optin.ensure(&f, 1, 100, set);
-          optin.ensure(&f, 0, 100, set);
-          optin.ensure(&f, 1, 90, set);
-          optin.ensure(&f, 1, 101, set);
+          for (int i : {0, 1, 0}) optin.ensure(&f, i, 100, set, 2);
+          optin.ensure(&f, 1, 90, set, 2);
+          optin.ensure(&f, 1, 101, set, 2);
           return n;
         }''')
     calls = ctypes.c_int()
@@ -303,3 +301,59 @@ def test_cpp_launchers_pass_their_arguments_in_order(tmp_path):
     include = os.path.join(os.path.dirname(PKG), "include")
     assert host_library(tmp_path, source, f"-I{include}", f"-L{lib}", f"-Wl,-rpath,{lib}",
                         "-l:libflash_engine_b200.so").run() == 0
+
+
+def test_bookkeeping_throws_nothing_through_the_c_entries(tmp_path):
+    """Without memory for a record: a status, and every stream counted as one to wait for."""
+    lib = host_library(tmp_path, '''
+        #include <cstdlib>
+        #include <new>
+        static bool none = false;
+        void* take(std::size_t n) {
+          if (none) throw std::bad_alloc();
+          return std::malloc(n);
+        }
+        template <typename T>
+        struct Failing {  // in place of std::allocator in the two headers
+          using value_type = T;
+          Failing() = default;
+          template <typename U> Failing(const Failing<U>&) {}
+          T* allocate(std::size_t n) { return static_cast<T*>(take(n * sizeof(T))); }
+          void deallocate(T* p, std::size_t) { std::free(p); }
+          template <typename U> bool operator==(const Failing<U>&) const { return true; }
+          template <typename U> bool operator!=(const Failing<U>&) const { return false; }
+        };
+        #include <algorithm>
+        #include <atomic>
+        #include <map>
+        #include <mutex>
+        #include <utility>
+        #include <vector>
+        namespace poor {
+        template <typename T> using vector = std::vector<T, Failing<T>>;
+        template <typename K, typename V>
+        using map = std::map<K, V, std::less<K>, Failing<std::pair<const K, V>>>;
+        }
+        namespace std { namespace host_test { using poor::vector; using poor::map; } }
+        #define vector host_test::vector
+        #define map host_test::map
+        #include "launch_order.h"
+        #include "smem_optin.h"
+        #undef vector
+        #undef map
+        extern "C" int run() {
+          static fe::TableWriters w;
+          static fe::SmemOptin o;
+          auto set = [](int) { return 0; };
+          int f = 0, n = 0;
+        #define CHECK(x) ++n; if (!(x)) return n;
+          CHECK(o.ensure(&f, 0, 100, set, 2) == 0 && !w.passed(0, nullptr))
+          none = true;
+          CHECK(o.ensure(&f, 1, 100, set, 2) == 2 && o.ensure(&f, 0, 200, set, 2) == 0)
+          w.wrote(0, nullptr);
+          CHECK(w.passed(0, nullptr) && w.passed(0, &f) && w.passed(1, nullptr))
+          none = false;
+          CHECK(o.ensure(&f, 1, 100, set, 2) == 0 && w.passed(0, nullptr))
+          return 0;
+        }''')
+    assert lib.run() == 0
